@@ -1,0 +1,142 @@
+// What the attention kernels over the 8-bit cache share: their arguments, which tile a block works on, and conversions.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace {
+constexpr int D = HEAD_DIM;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Kv8Args {
+    const unsigned char* k_cache;
+    const unsigned char* v_cache;
+    const float* k_scale;    // [num_pages, KV]
+    const float* v_scale;
+    const int* cu_q;         // [n + 1] start of each request's new tokens
+    const int* ctx_lens;     // [n] tokens in the cache, the new ones among them
+    const int* block_table;  // [n, table_width]
+    int n, n_tokens, table_width, page_size, num_pages;
+    int page_shift;          // log2(page_size) when it is a power of two, else -1
+    long long page_stride;   // bytes from page to page
+    long long q_stride;      // entries from token to token
+    int H, KV;
+    int heads_per_tile;      // query heads of one KV head that a tile handles
+    int tokens_per_tile;
+    int head_groups;         // tiles that the heads of one KV head make
+    float scale;
+    int window;              // 0: unlimited
+    int min_q, max_q;        // requests of so many new tokens are worked on
+    int any_q;               // no request brings more
+    int* status;
+
+    __device__ __forceinline__ int page_of(int key) const { return page_shift >= 0 ? key >> page_shift : key / page_size; }
+    __device__ __forceinline__ int in_page(int key) const { return page_shift >= 0 ? key & (page_size - 1) : key % page_size; }
+};
+
+inline Kv8Args kv8_args(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, const int* cu_q, const int* ctx_lens,
+                        const int* block_table, int n, int n_tokens, int table_width, int page_size, long long page_stride, int num_pages, int H, int KV,
+                        long long q_stride, float scale, int window, int min_q, int max_q, int any_q, int tile_rows, int* status) {
+    Kv8Args a;
+    a.k_cache = (const unsigned char*)k_cache;
+    a.v_cache = (const unsigned char*)v_cache;
+    a.k_scale = k_scale;
+    a.v_scale = v_scale;
+    a.cu_q = cu_q;
+    a.ctx_lens = ctx_lens;
+    a.block_table = block_table;
+    a.n = n;
+    a.n_tokens = n_tokens;
+    a.table_width = table_width;
+    a.page_size = page_size;
+    a.num_pages = num_pages;
+    a.page_shift = -1;
+    for (int s = 0; s < 30; ++s)
+        if (page_size == 1 << s) a.page_shift = s;
+    a.page_stride = page_stride;
+    a.q_stride = q_stride;
+    a.H = H;
+    a.KV = KV;
+    const int group = H / KV;
+    a.heads_per_tile = group < tile_rows ? group : tile_rows;
+    a.tokens_per_tile = tile_rows / a.heads_per_tile;
+    a.head_groups = (group + a.heads_per_tile - 1) / a.heads_per_tile;
+    a.scale = scale;
+    a.window = window;
+    a.min_q = min_q;
+    a.max_q = max_q;
+    a.any_q = any_q;
+    a.status = status;
+    return a;
+}
+
+struct Kv8Tile {
+    int req;       // -1: no such tile
+    int q_begin;   // the request's first row of q
+    int q_len;
+    int tok0;      // the tile's first token, counted from the request's first new one
+};
+
+// The `index`-th tile over all requests, in their order: each warp of a block finds it for itself from the boundaries, so that neither host nor
+// an earlier kernel has to make a list. With one token a request at most, tile and request are one. `look`: this block also checks
+// that no request brings more than `any_q` tokens.
+__device__ __forceinline__ Kv8Tile kv8_find_tile(const Kv8Args& a, int index, int tokens_per_tile, bool look) {
+    Kv8Tile t = {-1, 0, 0, 0};
+    const int lane = threadIdx.x & 31;
+    if (a.any_q == 1) {
+        if (index >= a.n) return t;
+        const int from = __ldg(a.cu_q + index), len = __ldg(a.cu_q + index + 1) - from;
+        if (len < 1) return t;
+        if (len > 1 || from < 0 || from >= a.n_tokens) {
+            if (threadIdx.x == 0) oxr_report(a.status, OXR_BAD_ARGUMENT, index);
+            return t;
+        }
+        t.req = index; t.q_begin = from; t.q_len = 1;
+        return t;
+    }
+    int before = 0;
+    for (int r0 = 0; r0 < a.n; r0 += 32) {
+        const int r = r0 + lane;
+        const int from = r < a.n ? __ldg(a.cu_q + r) : 0, len = r < a.n ? __ldg(a.cu_q + r + 1) - from : 0;
+        const bool bad = len > a.any_q || (len > 0 && (from < 0 || (long long)from + len > a.n_tokens));
+        if (look && bad && threadIdx.x < 32) oxr_report(a.status, OXR_BAD_ARGUMENT, r);
+        const int count = (!bad && len >= a.min_q && len <= a.max_q) ? (len + tokens_per_tile - 1) / tokens_per_tile : 0;
+        int upto = count;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const int mine = index - before - (upto - count);
+        const unsigned hit = __ballot_sync(0xffffffffu, mine >= 0 && mine < count);
+        if (hit && t.req < 0) {
+            const int src = __ffs(hit) - 1;
+            t.req = r0 + src;
+            t.q_begin = __shfl_sync(0xffffffffu, from, src);
+            t.q_len = __shfl_sync(0xffffffffu, len, src);
+            t.tok0 = __shfl_sync(0xffffffffu, mine, src) * tokens_per_tile;
+            if (!look) break;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return t;
+}
+
+// Two e4m3 codes (the low 16 bits) as two fp16 numbers: exact, NaN stays NaN.
+__device__ __forceinline__ uint32_t codes_to_f16(uint32_t w) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(w));
+    return r;
+}
+// The integer e with 2^(e - 1) < s <= 2^e for a positive finite s (subnormal ones count as 2^-126).
+__device__ __forceinline__ int scale_exponent(float s) {
+    const uint32_t b = __float_as_uint(s);
+    return max((int)(b >> 23) - 127 + ((b & 0x7fffffu) != 0), -126);
+}
+__device__ __forceinline__ float exp2_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+}  // namespace

@@ -46,6 +46,9 @@ enum OxrStatus : int {
     OXR_BAD_POSITION = 3,     // position outside the rotary table
     OXR_BAD_PAGE = 4,         // attention: block table names a page outside the pool
     OXR_WAIT_EXPIRED = 5,     // a bounded wait on an mbarrier ran out
+    OXR_NO_PAGES = 6,         // page tables: the step needs more pages than are free
+    OXR_LONG_REQUEST = 7,     // page tables: a row's numbers do not fit it (a request longer than its row of the block table, a negative length)
+    OXR_MANY_TOKENS = 8,      // page tables: more new tokens than the step's arrays take
     OXR_BAD_ARGUMENT = 100,   // launcher refused its arguments (host side)
 };
 

@@ -33,6 +33,8 @@ runs) instead of the register-fed skinny kernel. ``OXR_B200_STREAM=0`` switches 
 STATUS_NAMES = {
     1: "token id outside the vocabulary", 2: "cache slot outside the pool", 3: "position outside the rotary table",
     4: "block table names a page outside the pool", 5: "a bounded wait inside a kernel ran out",
+    6: "a step needs more pages than are free", 7: "a request does not fit its row of the block table", 8: "a step brings more tokens than its arrays take",
+    100: "a kernel was given numbers that contradict its other arguments",
 }
 _DT = {torch.float32: 0, torch.bfloat16: 1}
 
@@ -2451,3 +2453,6 @@ def diff_combine(o: torch.Tensor, num_heads: int, value_dim: int, lam: torch.Ten
     _done(_lib().oxr_diff_combine(out.data_ptr(), o.data_ptr(), n, width, int(num_heads), int(value_dim), lam.data_ptr(), float(eps), float(factor),
                                   _dtype_code(o), _stream()), "diff_combine")
     return out
+
+
+from oxr_inference_b200.ops.kv8 import KV8_DTYPE, PageStep, paged_attention_kv8, step_pages, store_kv8  # noqa: E402, F401

@@ -1,7 +1,7 @@
 """Compiles the CUDA sources under ``csrc/`` for sm_100a with nvcc and loads them with ctypes.
 
-Two kinds of library: ``core`` (everything whose code does not depend on a model size) and ``attn_d<D>``
-(the attention kernels, compiled for one head size). A library is compiled at its first use, so a model folder
+Three kinds of library: ``core`` (everything whose code does not depend on a model size), ``attn_d<D>``
+(the attention kernels, compiled for one head size) and ``attn_kv8_d<D>`` (those over the 8-bit cache). A library is compiled at its first use, so a model folder
 costs only what that model needs; ``build_all`` compiles a given list up front. Objects are compiled in
 parallel, a progress line goes to stderr every few seconds, and the result is kept beside the sources
 (``csrc/_build``) when that folder can be written, else in a per-user folder under the system's temp
@@ -29,9 +29,10 @@ ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
 
 CORE_SOURCES = ["elementwise.cu", "qk_norm_rope.cu", "gemm_f32.cu", "gemm_f32_short.cu", "gemm_skinny.cu", "gemm_stream.cu", "gemm_tcgen05.cu", "gemm_tcgen05_pair.cu", "gemm_tcgen05_few_rows.cu", "sampling.cu",
-                "stream_ops.cu", "mamba.cu", "attention_rows.cu", "attention_mix.cu", "attention_mix_mma.cu", "conv_qkv.cu", "mlstm.cu", "experts.cu", "head_prep.cu", "gla.cu", "shift_norm.cu", "delta.cu", "differential.cu", "hyper.cu"]
+                "stream_ops.cu", "mamba.cu", "attention_rows.cu", "attention_mix.cu", "attention_mix_mma.cu", "conv_qkv.cu", "mlstm.cu", "experts.cu", "head_prep.cu", "gla.cu", "shift_norm.cu", "delta.cu", "differential.cu", "hyper.cu", "kv8.cu"]
 ATTENTION_SOURCES = ["attention.cu"]
-HEADERS = ["common.cuh", "scan_columns.cuh", "tma.cuh", "umma.cuh", "sampling_static.h"]
+KV8_SOURCES = ["attention_kv8.cu"]
+HEADERS = ["attention_kv8.cuh", "common.cuh", "scan_columns.cuh", "tma.cuh", "umma.cuh", "sampling_static.h"]
 
 
 TIMELINE = os.environ.get("OXR_B200_TIMELINE") == "1"
@@ -192,10 +193,16 @@ def attention_library(head_dim: int) -> ctypes.CDLL:
     return _load(name, _existing(ATTENTION_SOURCES), defines)
 
 
+def kv8_library(head_dim: int) -> ctypes.CDLL:
+    check_head_dim(head_dim)
+    return _load(f"attn_kv8_d{head_dim}", _existing(KV8_SOURCES), [f"-DHEAD_DIM={head_dim}"])
+
+
 def build_all(head_dims: tuple[int, ...] = (16, 32, 64, 128)) -> list[Path]:
-    """Compile the core library and the attention library of each head size; returns the library paths."""
+    """Compile the core library and the attention libraries of each head size; returns the library paths."""
     out = [_compile("core", _existing(CORE_SOURCES), [])]
     for d in head_dims:
         check_head_dim(d)
         out.append(_compile(f"attn_d{d}", _existing(ATTENTION_SOURCES), [f"-DHEAD_DIM={d}"]))
+        out.append(_compile(f"attn_kv8_d{d}", _existing(KV8_SOURCES), [f"-DHEAD_DIM={d}"]))
     return out
