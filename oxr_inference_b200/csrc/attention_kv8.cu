@@ -5,19 +5,25 @@
 // of its request sees the keys j <= p (j > p - window behind a window):
 //     s_j = scale * ks_j * (q . K_j),     o = sum_j exp(s_j) vs_j V_j / sum_j exp(s_j).
 //
-// Every e4m3 number is an fp16 number, so the codes go through the tensor cores as they are (mma.sync m16n8k16, fp16 operands, fp32 sums; a
-// pair of codes costs one conversion, 64 lanes a clock) and both scales stay outside the products: ks multiplies the fp32 score, vs the weight.
-// A bf16 query is an fp16 number too once its row is multiplied by a power of two that brings its largest entry to 2^14 (entries 2^-39
-// below that are lost); an fp32 query is the sum of two fp16 numbers to 22 bits. The weights are rounded to fp16 (11 bits) against the row's
-// running maximum, times 2^15 so that they keep their bits down to 2^-29 of it; with fp32 queries they too are two numbers.
+// The codes go through the tensor cores as they are (mma.sync, fp32 sums) and both scales stay outside the products: ks multiplies the fp32 score,
+// vs the weight. Keys and values are the left operands (16 keys, or 16 entries of the values, by the products' depth) and the queries the right one (8
+// of them): a decode step has as few queries per KV head as that, and scores, weights and sums then come in fragments of 8 columns, a half of what
+// 16 rows of queries would take.
+// Every code is an fp16 number (a pair costs one conversion, 64 lanes a clock), so both products are m16n8k16 on fp16 operands. (m16n8k32 takes codes
+// as they are, but converts them itself, again for each product: scores that way, with the queries as two e4m3 numbers, took 76 us where fp16 took 68.)
+// A bf16 query is an fp16 number too once its row is multiplied by a power of two that brings its largest entry to 2^14 (what lies 2^-39 below that is
+// lost); an fp32 query is the sum of two fp16 numbers to 22 bits. The weights are rounded to fp16 (11 bits) against the row's running maximum, times
+// 2^15 so that they keep their bits down to 2^-29 of it; with fp32 queries they are two numbers as well.
 //
 // The weights of a block of keys are taken against the maximum of s_j + log2(vs) instead of s_j: weights times scales then never exceed one
 // however much the scales of pages differ, and a rescaled sum needs nothing but the usual factor. (log2(vs) stands for the integer 2^lv >= the
 // block's largest scale, relative to the scale of the last page, so that neither sums nor weights leave the fp32 range.)
 //
-// Each warp walks over blocks of 32 keys of its own: a ring of three stages filled with cp.async, one online softmax per warp, no block-wide barrier
-// until the end, where the warps' results are joined in shared memory and those of the blocks of a cluster (which share one request's keys when
-// there are few requests) through distributed shared memory. What bounds it is reading the cache: 2 D bytes per key and KV head.
+// The work is a row of items, one for each block of 32 keys of each tile (rows of queries of one KV head) of each request, and every warp of the
+// grid takes an equal stretch of it, so that requests of any lengths keep all of them busy to the end; the boundaries are worked out on the GPU, from
+// the lengths. A warp is on its own: a ring of stages filled by TMA (with cp.async where pages are not multiples of eight keys), one online softmax,
+// no barrier. What it has of a tile that it does not have whole goes to scratch memory, and a second kernel joins those pieces. What bounds it
+// is reading the cache: 2 D bytes per key and KV head.
 #include <cuda_fp16.h>
 
 #include "tma.cuh"
@@ -30,26 +36,49 @@ static_assert(HEAD_DIM % 16 == 0 && HEAD_DIM >= 16 && HEAD_DIM <= 256, "head siz
 #include "attention_kv8.cuh"
 
 namespace {
-constexpr int ROWS = 16;                       // rows of a tile: (token, query head) pairs of one KV head
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 constexpr int KEYS = 32;                       // keys of a block: one per lane while addresses are worked out
-constexpr int STAGES = D <= 64 ? 4 : 3;
-constexpr int PITCH = (D / 16) % 2 ? D : D + 16;   // bytes from key to key: an odd number of 16-byte words, so that eight rows lie on different banks
-constexpr int STAGE_BYTES = 2 * KEYS * PITCH + 2 * KEYS * 4;
+// A stage holds K and V as panels of PW bytes a key. Where a row is an odd number of 16-byte words it is a panel of its own and eight rows lie on
+// different banks as they are; elsewhere panels are the largest power of two up to 128 bytes and swizzled as TMA does it.
+constexpr bool SWIZZLED = (D / 16) % 2 == 0;
+constexpr int PW = !SWIZZLED ? D : (D % 128 == 0 ? 128 : D % 64 == 0 ? 64 : 32);
+constexpr int PANELS = D / PW;
+constexpr int TENSOR_BYTES = KEYS * D;
+constexpr int STAGE_BYTES = 2 * TENSOR_BYTES;      // a multiple of 1,024: swizzled panels start where the pattern does
+constexpr int SCALE_BYTES = 2 * KEYS * 4;
 constexpr int KSTEPS = D / 16;
-constexpr int RING_BYTES = WARPS * STAGES * STAGE_BYTES;
-constexpr int PART_BYTES = ROWS * D * 4;       // a warp's sums when they are joined: they take the place of its ring
-static_assert(PART_BYTES <= STAGES * STAGE_BYTES, "the sums of a warp fit into its ring");
 constexpr float P_FACTOR = 32768.f;            // weights are kept as 2^15 w
-
-template <int PIECES> __host__ __device__ constexpr bool q_in_regs() { return PIECES * D <= 256; }
-template <int PIECES> constexpr size_t smem_bytes() {
-    return RING_BYTES + WARPS * ROWS * 8 + ROWS * 8 + (q_in_regs<PIECES>() ? 0 : PIECES * KSTEPS * 512);
-}
+constexpr int GROUPS = 2 * THREADS, GROUP_BYTES = (GROUPS + 2 + WARPS) * 8;   // see Items
+// Of a kernel whose tiles have 8 NQ rows, (token, query head) pairs of one KV head:
+template <typename T, int NQ> struct Shape {
+    static constexpr int PIECES = sizeof(T) == 4 ? 2 : 1;             // fp16 numbers that make a query's entry or a weight
+    static constexpr int ROWS = 8 * NQ;
+    static constexpr int Q_WORDS = NQ * KSTEPS * PIECES * 2;          // of a lane
+    static constexpr bool Q_IN_REGS = Q_WORDS + NQ * D / 4 <= 160;    // beside the sums
+    // Blocks of four warps on an SM: with 8 rows of bf16 queries the registers suffice for three, which hide more of each other's waits than a third
+    // stage does (64 requests of 2,048 keys: 59 against 68 us); the ring takes what shared memory that leaves, four stages at most.
+    static constexpr int BLOCKS = D > 128 ? 1 : NQ == 1 && PIECES == 1 ? 3 : 2;
+    static constexpr int FIT = (225 * 1024 / BLOCKS - 4096 - (Q_IN_REGS ? 0 : WARPS * Q_WORDS * 128)) / (WARPS * (STAGE_BYTES + SCALE_BYTES));
+    static constexpr int STAGES = FIT < 4 ? FIT : 4;
+    static_assert(STAGES >= 2, "room for a ring");
+    static constexpr int RING_BYTES = WARPS * STAGES * STAGE_BYTES;
+    static constexpr int AT_BARS = RING_BYTES + WARPS * STAGES * SCALE_BYTES, AT_GROUPS = AT_BARS + WARPS * STAGES * 8, AT_Q = AT_GROUPS + GROUP_BYTES;
+    static constexpr size_t SMEM = AT_Q + (Q_IN_REGS ? 0 : WARPS * Q_WORDS * 128);
+    static_assert(SMEM <= 227 * 1024, "shared memory of a block");
+};
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+// What the swizzle of a panel's row changes in the address of its 16-byte words.
+__device__ __forceinline__ uint32_t row_swizzle(int row) {
+    return !SWIZZLED ? 0u : PW == 128 ? (uint32_t)(row & 7) << 4 : PW == 64 ? (uint32_t)((row >> 1) & 3) << 4 : (uint32_t)((row >> 2) & 1) << 4;
+}
+// The address of 16-byte word `w` of a row, from that of the row in the first panel with the row's swizzle in it.
+__device__ __forceinline__ uint32_t word_at(uint32_t row, int w) {
+    if constexpr (!SWIZZLED) return row + w * 16;
+    return (row ^ (uint32_t)(w % (PW / 16) * 16)) + (uint32_t)(w / (PW / 16) * KEYS * PW);
 }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool take) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4 : 0) : "memory");
@@ -67,31 +96,12 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t cluster_rank() {
+// An 8 x 8 matrix of 16-bit numbers, two of a row per lane, turned over.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-    return v;
-}
-
 // Four entries of a query row.
 __device__ __forceinline__ float4 load4(const float* p) { return __ldg(reinterpret_cast<const float4*>(p)); }
 __device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
@@ -105,6 +115,20 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
     reinterpret_cast<__nv_bfloat162*>(&w)[1] = __floats2bfloat162_rn(v.z, v.w);
     *reinterpret_cast<uint2*>(p) = w;
 }
+__device__ __forceinline__ void store2(float* p, float2 v) { *reinterpret_cast<float2*>(p) = v; }
+__device__ __forceinline__ void store2(__nv_bfloat16* p, float2 v) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v.x, v.y); }
+// (top, total, v) += another maximum, sum and its entries. A sum of nothing has neither; a NaN may have a sum without a maximum and stays.
+template <int PER> __device__ __forceinline__ void add_piece(float& top, float& total, float4 (&v)[PER], float2 ml, const float4 (&u)[PER]) {
+    if (ml.y == 0.f) return;
+    const float n = fmaxf(top, ml.x), f0 = top == n ? 1.f : exp2_of(top - n), f1 = ml.x == n ? 1.f : exp2_of(ml.x - n);
+    top = n;
+    total = total * f0 + ml.y * f1;
+#pragma unroll
+    for (int x = 0; x < PER; ++x) {
+        v[x].x = v[x].x * f0 + u[x].x * f1; v[x].y = v[x].y * f0 + u[x].y * f1;
+        v[x].z = v[x].z * f0 + u[x].z * f1; v[x].w = v[x].w * f0 + u[x].w * f1;
+    }
+}
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -115,45 +139,169 @@ __device__ __forceinline__ uint32_t pack_rest(float lo, float hi, uint32_t packe
     return pack_f16(lo - f.x, hi - f.y);
 }
 
-// One tile of ROWS rows. The walk over the keys is cut between the blocks of a cluster (`splits` of them) and their warps.
-template <typename T>
-__global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1)
-attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const Kv8Args a, const int splits) {
-    constexpr int PIECES = sizeof(T) == 4 ? 2 : 1;
-    constexpr bool QREG = q_in_regs<PIECES>();
-    extern __shared__ __align__(16) unsigned char smem[];
-    float2* warp_ml = reinterpret_cast<float2*>(smem + RING_BYTES);            // [WARPS][ROWS] running maximum and sum
-    float2* block_ml = warp_ml + WARPS * ROWS;                                // [ROWS]
-    [[maybe_unused]] uint4* q_smem = reinterpret_cast<uint4*>(block_ml + ROWS);   // [PIECES][KSTEPS][32 lanes]
+// ---- the row of work items
+// Request after request; of a request tile after tile, of a tile each group of query heads (`per_tile` of them), of that the blocks of 32 keys behind
+// TILE_COST items that stand for the time a warp needs to begin a tile and to put its result away (without them a warp whose stretch is a dozen of
+// requests of a few tokens works twice as long as the others: 24 requests of 1 to 32,768 keys 118 us without,
+// 79 with one, 66 with three). All tiles of a request count as many blocks as the widest; what a tile lacks of them is empty. A block of threads sums up the items of 256 groups of neighbouring
+// requests (each request is its own group up to 256 of them); a warp finds the request of an item by bisection and a scan of the group.
+constexpr int TILE_COST = 3;
+struct Items {
+    const Kv8Args& a;
+    long long* upto;        // [GROUPS + 1] in shared memory: items of the groups before
+    int group, per_tile;
+
+    struct Request { int q_begin, q_len, ctx, tiles, blocks; long long items; };
+    __device__ __forceinline__ Request request(int r, bool look) const {
+        Request x = {0, 0, 0, 0, 1, 0};
+        if (r >= a.n) return x;
+        x.q_begin = __ldg(a.cu_q + r);
+        x.q_len = __ldg(a.cu_q + r + 1) - x.q_begin;
+        x.ctx = __ldg(a.ctx_lens + r);
+        if (x.q_len < 1) return x;
+        if (x.q_len > a.any_q || x.q_begin < 0 || (long long)x.q_begin + x.q_len > a.n_tokens) {
+            if (look) oxr_report(a.status, OXR_BAD_ARGUMENT, r);
+            return x;
+        }
+        if (x.q_len < a.min_q || x.q_len > a.max_q) return x;
+        x.tiles = (x.q_len + a.tokens_per_tile - 1) / a.tokens_per_tile;
+        const int keys = min((long long)max(x.ctx, 0), (long long)a.table_width * a.page_size);
+        x.blocks = max(1, (keys + KEYS - 1) / KEYS);
+        if (a.window > 0) x.blocks = min(x.blocks, (int)(((long long)a.window + a.tokens_per_tile + KEYS - 2) / KEYS) + 1);
+        x.blocks += TILE_COST;
+        x.items = (long long)x.tiles * per_tile * x.blocks;
+        return x;
+    }
+    // All items; by every thread of the block. `sums`: a word of shared memory per warp.
+    __device__ long long prepare(long long* sums) {
+        group = (a.n + GROUPS - 1) / GROUPS;
+        per_tile = a.KV * a.head_groups;
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        long long mine[2] = {0, 0};                // a thread's two groups, side by side
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            for (int r = 0; r < group; ++r) mine[k] += request((threadIdx.x * 2 + k) * group + r, blockIdx.x == 0).items;
+        long long v = mine[0] + mine[1];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long w = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += w;
+        }
+        if (lane == 31) sums[warp] = v;
+        __syncthreads();
+        long long before = v - mine[0] - mine[1], all = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const long long s = sums[w];
+            if (w < warp) before += s;
+            all += s;
+        }
+        upto[threadIdx.x * 2] = before;
+        upto[threadIdx.x * 2 + 1] = before + mine[0];
+        if (threadIdx.x == 0) upto[GROUPS] = all;
+        __syncthreads();
+        return all;
+    }
+    struct Place { int req; Request of; int tile, y, block; };
+    // Of item `i`, which is one; by a whole warp.
+    __device__ __forceinline__ Place find(int i) const {
+        int low = 0, high = GROUPS;               // the last group that begins at or before it (those without items share their start with the next)
+        while (high - low > 1) {
+            const int mid = (low + high) >> 1;
+            if (upto[mid] <= i) low = mid; else high = mid;
+        }
+        int rest = i - (int)upto[low];
+        Place p;
+        p.req = low * group;
+        p.of = request(p.req, false);
+        for (int r = 1; r < group && rest >= p.of.items; ++r) {
+            rest -= (int)p.of.items;
+            p.of = request(++p.req, false);
+        }
+        const int per = p.of.blocks * per_tile;
+        p.tile = rest / per;
+        const int in_tile = rest - p.tile * per;
+        p.y = in_tile / p.of.blocks;
+        p.block = in_tile % p.of.blocks;
+        return p;
+    }
+};
+
+// Scratch: a warp leaves what it has of a tile in its first place when the tile began before its stretch, else in its second.
+struct Cut {         // what the join has to know of a tile that a stretch ends in and that began in it
+    int last;        // the warp with its last piece; -1: the stretch ends in no such tile
+    int token, head; // first row of q and first head
+    int rows, heads; // (token, head) pairs of the tile, and how many heads of them there are
+    int base_exp;    // what the pieces are relative to
+    int spare[2];
+};
+struct Pieces {
+    float* sums;     // [2 * warps][ROWS][D]
+    float2* ml;      // [2 * warps][ROWS] running maximum and sum
+    Cut* cuts;       // [warps]
+};
+
+// TMA: pages hold whole pieces of 8, 16 or 32 keys (2^piece_shift), which come in as boxes; otherwise each lane copies 16 bytes at a time.
+template <typename T, bool TMA, int NQ>
+__global__ void __launch_bounds__(THREADS, Shape<T, NQ>::BLOCKS)
+attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                const int piece_shift, const Kv8Args a, const Pieces left) {
+    using S = Shape<T, NQ>;
+    constexpr int ROWS = S::ROWS, PIECES = S::PIECES, STAGES = S::STAGES, SCALES_AT = S::RING_BYTES;
+    extern __shared__ __align__(1024) unsigned char smem[];   // nothing static stands before it: it starts on a 1,024-byte boundary
+    long long* groups = reinterpret_cast<long long*>(smem + S::AT_GROUPS);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, quad = lane & 3;
+    if (TMA && threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+    }
+    const uint32_t ring = smem_addr(smem) + warp * STAGES * STAGE_BYTES, my_scales = smem_addr(smem) + SCALES_AT + warp * STAGES * SCALE_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::AT_BARS) + warp * STAGES;   // a stage's rows have arrived
+    [[maybe_unused]] uint32_t* q_smem = reinterpret_cast<uint32_t*>(smem + S::AT_Q) + warp * S::Q_WORDS * 32;   // [Q_WORDS][32 lanes]
+    if (TMA && lane == 0) {
+        for (int i = 0; i < STAGES; ++i) mbar_init(bars + i, 1);
+        mbar_fence_init();
+        fence_proxy_async();
+    }
     pdl_wait();
     pdl_trigger();
+    Items items = {a, groups};
+    const long long all = items.prepare(groups + GROUPS + 2);
+    const int G = a.H / a.KV, me = (int)blockIdx.x * WARPS + warp;
+    const int warps = (int)gridDim.x * WARPS;
+    if (all > 0x7fffffffll - warps) {      // some thousands of the longest sequences: more than a step can mean
+        if (blockIdx.x == 0 && threadIdx.x == 0) oxr_report(a.status, OXR_BAD_ARGUMENT, -1);
+        if (lane == 0) left.cuts[me].last = -1;
+        return;
+    }
+    const int share = max(1, ((int)all + warps - 1) / warps), end = (int)min(all, (me + 1ll) * share);
+    int turn = 0;      // stages filled before this tile: the ring and its barriers go on from there
+    Cut cut = {-1, 0, 0, 0, 0, 0, {0, 0}};
+
+    for (int item = (int)min(all, (long long)me * share); item < end;) {
+    const Items::Place at = items.find(item);
+    const int count = min(end - item, at.of.blocks - at.block);   // items of this tile that are this warp's
+    item += count;
 
     // ---- which rows
-    const int unit = (int)(blockIdx.x / (unsigned)splits), rank = splits > 1 ? (int)cluster_rank() : 0;
-    const int per_tile = a.KV * a.head_groups;
-    const int y = unit % per_tile, kvh = y / a.head_groups, hg = y % a.head_groups;
-    const Kv8Tile t = kv8_find_tile(a, unit / per_tile, a.tokens_per_tile, unit == 0);
-    if (t.req < 0) return;                    // the same for every block of a cluster
-    const int q_len = t.q_len, tok0 = t.tok0;
-    const int tokens = min(a.tokens_per_tile, q_len - tok0);
-    const int ctx = __ldg(a.ctx_lens + t.req), pos0 = ctx - q_len;   // position of the request's first new token
+    const int kvh = at.y / a.head_groups, hg = at.y % a.head_groups;
+    const int q_begin = at.of.q_begin, tok0 = at.tile * a.tokens_per_tile;
+    const int tokens = min(a.tokens_per_tile, at.of.q_len - tok0);
     const int rows = tokens * a.heads_per_tile;
-    const int G = a.H / a.KV;
-    const int first_pos = pos0 + tok0, last_pos = first_pos + tokens - 1;
+    const int first_pos = at.of.ctx - at.of.q_len + tok0, last_pos = first_pos + tokens - 1;
     int hi = last_pos + 1;
     const int lo = a.window > 0 ? max(0, first_pos - a.window + 1) : 0;
     if (hi > (long long)a.table_width * a.page_size) {
-        if (threadIdx.x == 0) oxr_report(a.status, OXR_BAD_PAGE, t.req);
+        if (lane == 0) oxr_report(a.status, OXR_BAD_PAGE, at.req);
         hi = a.table_width * a.page_size;
     }
-    const int block0 = max(lo, 0) / KEYS, blocks = hi > lo ? (hi + KEYS - 1) / KEYS - block0 : 0;
-    const int* table_row = a.block_table + (size_t)t.req * a.table_width;
-    const int walkers = splits * WARPS, me = rank * WARPS + warp;
+    const int block0 = lo / KEYS + max(0, at.block - TILE_COST), blocks_end = min(lo / KEYS + at.block + count - TILE_COST, hi > lo ? (hi + KEYS - 1) / KEYS : 0);
+    const int mine = max(0, blocks_end - block0);      // blocks of keys to visit
+    const int* table_row = a.block_table + (size_t)at.req * a.table_width;
 
     // the scale that scales are relative to: the last visible page's
     int base_exp = 0;
-    if (blocks > 0) {
+    if (hi > lo) {
         const int page = __ldg(table_row + a.page_of(hi - 1));
         if (page >= 0 && page < a.num_pages) {
             const float s = __ldg(a.v_scale + (size_t)page * a.KV + kvh);
@@ -162,31 +310,58 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const Kv8Args a, c
     }
 
     // ---- the keys' way into the ring
-    const uint32_t ring = smem_addr(smem) + warp * STAGES * STAGE_BYTES;
-    auto page_for = [&](int i) -> int {       // of this lane's key of the warp's i-th block; -1: nothing to fetch
-        const int key = (block0 + me + i * walkers) * KEYS + lane;
-        if (me + i * walkers >= blocks || key < lo || key >= hi) return -1;
+    bool bad_page = false;                    // the request's table named one: the result is void
+    auto page_for = [&](int i) -> int {       // of this lane's key of the i-th block; -1: nothing to fetch
+        const int key = (block0 + i) * KEYS + lane;
+        if (i >= mine || key < lo || key >= hi) return -1;
         return __ldg(table_row + a.page_of(key));
     };
+    // By TMA a lane sends for one panel of one piece of K or V, and a barrier counts what arrives; the scales of the lane's own key are a copy group.
     auto fetch = [&](int i, int page) {
-        if (me + i * walkers < blocks) {
-            const int key = (block0 + me + i * walkers) * KEYS + lane;
+        if (i < mine) {
+            const int key0 = (block0 + i) * KEYS, key = key0 + lane, slot = (turn + i) % STAGES;
             const bool wanted = key >= lo && key < hi, good = wanted && page >= 0 && page < a.num_pages;
-            if (wanted && !good) oxr_report(a.status, OXR_BAD_PAGE, t.req);
-            const long long row = good ? (long long)page * a.page_stride + ((long long)a.in_page(key) * a.KV + kvh) * D : -1;
-            const uint32_t st = ring + (i % STAGES) * STAGE_BYTES;
+            if (wanted && !good) oxr_report(a.status, OXR_BAD_PAGE, at.req);
+            if (TMA) bad_page |= __any_sync(0xffffffffu, wanted && !good);
+            const uint32_t st = ring + slot * STAGE_BYTES;
+            const int place = good ? page : -1;
+            if constexpr (TMA) {
+                // a piece is on one page: whichever of its keys are wanted name it
+                const unsigned some = __ballot_sync(0xffffffffu, good);
+                const int pieces = KEYS >> piece_shift, piece = 1 << piece_shift, ops = 2 * PANELS * pieces;
+                const unsigned mine = some >> ((lane & (pieces - 1)) << piece_shift) & (0xffffffffu >> (32 - piece));   // of the piece that this lane sends for
+                const int there = __popc(__ballot_sync(0xffffffffu, lane < pieces && mine));
+                uint64_t* bar = bars + slot;
+                if (lane == 0) {
+                    if (there) mbar_expect_tx(bar, (uint32_t)(there * piece * 2 * D));
+                    else mbar_arrive(bar);
+                }
+                __syncwarp();
+                for (int x0 = 0; x0 < ops; x0 += 32) {
+                    const int x = x0 + lane, pc = x & (pieces - 1), of = x >> (5 - piece_shift), pnl = of % PANELS;
+                    const bool is_v = of >= PANELS;
+                    const int from = __shfl_sync(0xffffffffu, place, pc * piece + (mine ? __ffs(mine) - 1 : 0));
+                    if (x < ops && mine)
+                        tma_load_3d(smem + (st - smem_addr(smem)) + is_v * TENSOR_BYTES + pnl * KEYS * PW + pc * piece * PW, is_v ? &map_v : &map_k,
+                                    kvh * D + pnl * PW, a.in_page(key0 + pc * piece), from, bar);
+                }
+            } else {
+                const long long row = good ? (long long)page * a.page_stride + (a.in_page(key) * a.KV + kvh) * D : -1;
 #pragma unroll
-            for (int c = 0; c < KSTEPS; ++c) {
-                const int chunk = c * 32 + lane, r = chunk / KSTEPS, col = chunk % KSTEPS;
-                const long long at = __shfl_sync(0xffffffffu, row, r);
-                const bool take = at >= 0;
-                const long long off = (take ? at : 0) + col * 16;
-                cp_async16(st + r * PITCH + col * 16, a.k_cache + off, take);
-                cp_async16(st + (KEYS + r) * PITCH + col * 16, a.v_cache + off, take);
+                for (int c = 0; c < KSTEPS; ++c) {
+                    const int chunk = c * 32 + lane, r = chunk / KSTEPS, col = chunk % KSTEPS;
+                    const long long from = __shfl_sync(0xffffffffu, row, r);
+                    const bool take = from >= 0;
+                    const long long off = (take ? from : 0) + col * 16;
+                    const uint32_t dst = word_at(st + r * PW ^ row_swizzle(r), col);
+                    cp_async16(dst, a.k_cache + off, take);
+                    cp_async16(dst + TENSOR_BYTES, a.v_cache + off, take);
+                }
             }
-            const size_t sc = good ? (size_t)page * a.KV + kvh : 0;
-            cp_async4(st + 2 * KEYS * PITCH + lane * 4, a.k_scale + sc, good);
-            cp_async4(st + 2 * KEYS * PITCH + (KEYS + lane) * 4, a.v_scale + sc, good);
+            const int sc = good ? page * a.KV + kvh : 0;
+            const uint32_t scale_at = my_scales + slot * SCALE_BYTES + lane * 4;
+            cp_async4(scale_at, a.k_scale + sc, good);
+            cp_async4(scale_at + KEYS * 4, a.v_scale + sc, good);
         }
         cp_async_commit();
     };
@@ -198,93 +373,129 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const Kv8Args a, c
         fetch(i, page);
     }
 
-    // ---- the queries: rows g and g + 8 of the tile, entries 16 kk + 4 quad .. + 3
-    bool row_ok[2];
-    int row_pos[2];
-    float row_factor[2];
-    uint32_t qa[QREG ? PIECES : 1][QREG ? KSTEPS : 1][4];
+    // ---- the queries: lane (g, quad) holds entries 16 c + 4 quad .. + 3 of rows g, g + 8, ...
+    uint32_t q_regs[S::Q_IN_REGS ? S::Q_WORDS : 1];
+    auto put_q = [&](int word, uint32_t v) {
+        if constexpr (S::Q_IN_REGS) q_regs[word] = v;
+        else q_smem[word * 32 + lane] = v;      // (a lane reads what it has written)
+    };
+    float row_factor[NQ][2];       // of rows 2 quad and 2 quad + 1, as the scores come
+    int row_pos[NQ][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int r = g + 8 * h, tok = r / a.heads_per_tile, head = hg * a.heads_per_tile + r % a.heads_per_tile;
-        row_ok[h] = r < rows && head < G;
-        row_pos[h] = first_pos + tok;
-        const T* src = q + (size_t)(t.q_begin + tok0 + tok) * a.q_stride + (size_t)(kvh * G + head) * D + 4 * quad;
+    for (int nq = 0; nq < NQ; ++nq) {
+        const int r = g + 8 * nq, tok = r / a.heads_per_tile, head = hg * a.heads_per_tile + r % a.heads_per_tile;
+        const bool row_ok = r < rows && head < G;   // (rows of the tile without a token or head hold zeros; what they compute goes nowhere)
+        const T* src = q + (size_t)(q_begin + tok0 + tok) * a.q_stride + (size_t)(kvh * G + head) * D + 4 * quad;
         float4 v[KSTEPS];
         float most = 0.f;
 #pragma unroll
-        for (int kk = 0; kk < KSTEPS; ++kk) {
-            v[kk] = row_ok[h] ? load4(src + 16 * kk) : make_float4(0.f, 0.f, 0.f, 0.f);
-            most = fmaxf(fmaxf(most, fmaxf(fabsf(v[kk].x), fabsf(v[kk].y))), fmaxf(fabsf(v[kk].z), fabsf(v[kk].w)));
+        for (int c = 0; c < KSTEPS; ++c) {
+            v[c] = row_ok ? load4(src + 16 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+            most = fmaxf(fmaxf(most, fmaxf(fabsf(v[c].x), fabsf(v[c].y))), fmaxf(fabsf(v[c].z), fabsf(v[c].w)));
         }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         // a power of two: the largest entry of the row goes to [2^14, 2^15)
         const int shift = (most > 0.f && most < INFINITY) ? min(14 - (int)((__float_as_uint(most) >> 23) & 255) + 127, 126) : 0;
         const float f = __uint_as_float((uint32_t)(shift + 127) << 23);
-        row_factor[h] = a.scale * LOG2E * __uint_as_float((uint32_t)(127 - shift) << 23);
+        const float factor = a.scale * LOG2E * __uint_as_float((uint32_t)(127 - shift) << 23);
 #pragma unroll
-        for (int kk = 0; kk < KSTEPS; ++kk) {
-            const uint32_t x = pack_f16(v[kk].x * f, v[kk].y * f), z = pack_f16(v[kk].z * f, v[kk].w * f);
-            uint32_t* q0 = QREG ? qa[0][QREG ? kk : 0] : reinterpret_cast<uint32_t*>(q_smem + kk * 32 + lane);
-            if (QREG || warp == 0) { q0[h] = x; q0[h + 2] = z; }
+        for (int c = 0; c < KSTEPS; ++c) {      // word 0: entries 4 quad, + 1; word 1: + 2, + 3
+            const float4 x = make_float4(v[c].x * f, v[c].y * f, v[c].z * f, v[c].w * f);
+            const uint32_t w0 = pack_f16(x.x, x.y), w1 = pack_f16(x.z, x.w);
+            put_q((nq * KSTEPS + c) * 2 * PIECES, w0);
+            put_q((nq * KSTEPS + c) * 2 * PIECES + 1, w1);
             if constexpr (PIECES == 2) {
-                uint32_t* q1 = QREG ? qa[PIECES - 1 < (QREG ? PIECES : 1) ? PIECES - 1 : 0][QREG ? kk : 0] : reinterpret_cast<uint32_t*>(q_smem + (KSTEPS + kk) * 32 + lane);
-                if (QREG || warp == 0) { q1[h] = pack_rest(v[kk].x * f, v[kk].y * f, x); q1[h + 2] = pack_rest(v[kk].z * f, v[kk].w * f, z); }
+                put_q((nq * KSTEPS + c) * 4 + 2, pack_rest(x.x, x.y, w0));
+                put_q((nq * KSTEPS + c) * 4 + 3, pack_rest(x.z, x.w, w1));
             }
         }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            row_factor[nq][e] = __shfl_sync(0xffffffffu, factor, (2 * quad + e) * 4);
+            row_pos[nq][e] = first_pos + (8 * nq + 2 * quad + e) / a.heads_per_tile;
+        }
     }
-    if constexpr (!QREG) __syncthreads();
-    const int row_lo0 = a.window > 0 ? row_pos[0] - a.window + 1 : 0, row_lo1 = a.window > 0 ? row_pos[1] - a.window + 1 : 0;
+    auto get_q = [&](int word) -> uint32_t {
+        if constexpr (S::Q_IN_REGS) return q_regs[word];
+        else return q_smem[word * 32 + lane];
+    };
     const int last_lo = a.window > 0 ? last_pos - a.window + 1 : 0;   // the latest start of a row's window
-    // (rows of the tile without a token or head hold zeros; what they compute goes nowhere)
 
-    float o[D / 8][4];
+    // sums: o[nq][m] holds entries 16 m + 2 g (words 0, 1) and 16 m + 2 g + 1 (words 2, 3) of rows 2 quad and 2 quad + 1
+    float o[NQ][KSTEPS][4];
+    float m[NQ][2], l[NQ][2];
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i)
+    for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        for (int i = 0; i < KSTEPS; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[nq][i][e] = 0.f;
+        m[nq][0] = m[nq][1] = -INFINITY;
+        l[nq][0] = l[nq][1] = 0.f;
+    }
 
     // ---- the walk
-    const int mine = blocks > me ? (blocks - me + walkers - 1) / walkers : 0;
     for (int i = 0; i < mine; ++i) {
         cp_async_wait<STAGES - 2>();
+        const int slot = (turn + i) % STAGES;
+        if (TMA && !mbar_wait(bars + slot, ((turn + i) / STAGES) & 1)) {
+            if (lane == 0) oxr_report(a.status, OXR_WAIT_EXPIRED, 40);
+            cp_async_wait<0>();
+            return;
+        }
         __syncwarp();
         {   // the stage that the block before this one has left
             const int page = next_page;
             next_page = page_for(i + STAGES);
             fetch(i + STAGES - 1, page);
         }
-        const uint32_t st = ring + (i % STAGES) * STAGE_BYTES;
-        const float* scales = reinterpret_cast<const float*>(smem + (st - smem_addr(smem)) + 2 * KEYS * PITCH);
-        const int key0 = (block0 + me + i * walkers) * KEYS;
-
-        // scores: four tiles of 8 keys
-        float c[4][4];
+        const uint32_t st = ring + slot * STAGE_BYTES;
+        const float* scales = reinterpret_cast<const float*>(smem + SCALES_AT + (warp * STAGES + slot) * SCALE_BYTES);
+        unsigned char* values = smem + (st - smem_addr(smem)) + TENSOR_BYTES;
+        const int key0 = (block0 + i) * KEYS;
+        if constexpr (TMA) {
+            // Values that no row sees but that lie in a piece which one does, or in one that was not fetched, become zero: a weight of zero does not
+            // undo a NaN. (Their scores are masked whatever the keys hold.)
+            const bool seen = key0 + lane >= lo && key0 + lane < hi;
+            if (__any_sync(0xffffffffu, !seen) || bad_page) {
+                if (!seen || bad_page) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) c[j][e] = 0.f;
-        const uint32_t k_addr = st + lane * PITCH;
-#pragma unroll
-        for (int kk = 0; kk < KSTEPS; ++kk) {
-            uint32_t w[4];
-            ldsm4(w, k_addr + kk * 16);
-            uint32_t b[4][2];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { b[j][0] = codes_to_f16(w[j]); b[j][1] = codes_to_f16(w[j] >> 16); }
-#pragma unroll
-            for (int pc = 0; pc < PIECES; ++pc) {
-                uint32_t qf[4];
-                if constexpr (QREG) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) qf[e] = qa[pc][kk][e];
-                } else {
-                    const uint4 v = q_smem[(pc * KSTEPS + kk) * 32 + lane];
-                    qf[0] = v.x; qf[1] = v.y; qf[2] = v.z; qf[3] = v.w;
+                    for (int c = 0; c < KSTEPS; ++c) *reinterpret_cast<uint4*>(values + c / (PW / 16) * KEYS * PW + lane * PW + c % (PW / 16) * 16) = make_uint4(0, 0, 0, 0);
                 }
+                __syncwarp();
+            }
+        }
+
+        // scores: two tiles of 16 keys by 8 rows; c[..][mt]: key 16 mt + g (words 0, 1) and + 8 (words 2, 3) of rows 2 quad and 2 quad + 1
+        float c[NQ][2][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) mma_f16(c[j], qf, b[j][0], b[j][1]);
+        for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[nq][mt][e] = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+            // lanes 0-7, 8-15, 16-23, 24-31 name keys 0-7 and 8-15 at 16-byte word 2 kk and again at 2 kk + 1
+            const uint32_t k_row = (st + (16 * mt + (lane & 15)) * PW) ^ row_swizzle(lane & 15) ^ (SWIZZLED ? (lane >> 4) * 16 : 0);
+#pragma unroll
+            for (int kk = 0; kk < (KSTEPS + 1) / 2; ++kk) {
+                uint32_t w[4];
+                ldsm4(w, word_at(k_row, 2 * kk) + (!SWIZZLED && 2 * kk + 1 < KSTEPS ? (lane >> 4) * 16 : 0));
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if (2 * kk + half >= KSTEPS) break;
+                    const uint32_t x = w[2 * half], z = w[2 * half + 1];
+                    const uint32_t kf[4] = {codes_to_f16(x), codes_to_f16(z), codes_to_f16_high(x), codes_to_f16_high(z)};
+#pragma unroll
+                    for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                        for (int pc = 0; pc < PIECES; ++pc) {
+                            const int word = ((nq * KSTEPS + 2 * kk + half) * PIECES + pc) * 2;
+                            mma_f16(c[nq][mt], kf, get_q(word), get_q(word + 1));
+                        }
+                }
             }
         }
         // the largest value scale of the block as a power of two, relative to the last page's
@@ -292,75 +503,102 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const Kv8Args a, c
         const uint32_t most_vs = __reduce_max_sync(0xffffffffu, (my_vs > 0.f && my_vs < INFINITY) ? __float_as_uint(my_vs) : 0u);
         const int lv = most_vs ? scale_exponent(__uint_as_float(most_vs)) - base_exp : 0;
         const float lvf = (float)lv;
-        const float v_inverse = exp2_of(-(float)(lv + base_exp));
-        // (c0, c1) row g, (c2, c3) row g + 8; keys 8 j + 2 quad, + 1
-        float mx0 = -INFINITY, mx1 = -INFINITY;
+        const float v_inverse = exp2_of(-(float)(lv + base_exp)), down = exp2_of(-lvf);
         const bool whole = key0 >= last_lo && key0 + KEYS - 1 <= min(first_pos, hi - 1);
+        float ks[4], vf[4];     // of keys g, g + 8, g + 16, g + 24
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float2 ks = *reinterpret_cast<const float2*>(scales + 8 * j + 2 * quad);
-            c[j][0] *= row_factor[0] * ks.x; c[j][1] *= row_factor[0] * ks.y;
-            c[j][2] *= row_factor[1] * ks.x; c[j][3] *= row_factor[1] * ks.y;
-            if (!whole) {
+            ks[j] = scales[g + 8 * j];
+            vf[j] = scales[KEYS + g + 8 * j] * v_inverse * P_FACTOR;   // at most 2^15
+        }
+        bool odd_scale = false;
+        if (!whole && tokens > 1) odd_scale = __any_sync(0xffffffffu, !(fabsf(my_vs) < INFINITY));
+        uint32_t p[NQ][PIECES][2][2];    // weights: [..][key tile][keys 0-7 or 8-15 of it]
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq) {
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int key = key0 + 8 * j + 2 * quad + e;
-                    if (key > row_pos[0] || key < row_lo0 || key >= hi) c[j][e] = -INFINITY;
-                    if (key > row_pos[1] || key < row_lo1 || key >= hi) c[j][2 + e] = -INFINITY;
+                    float& s = c[nq][j >> 1][(j & 1) * 2 + e];
+                    s *= row_factor[nq][e] * ks[j];
                 }
-            }
-            mx0 = fmaxf(mx0, fmaxf(c[j][0], c[j][1]));
-            mx1 = fmaxf(mx1, fmaxf(c[j][2], c[j][3]));
-        }
-        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-        const float n0 = fmaxf(m[0], mx0 + lvf), n1 = fmaxf(m[1], mx1 + lvf);
-        if (__any_sync(0xffffffffu, n0 > m[0] || n1 > m[1])) {
-            const float a0 = n0 > m[0] ? exp2_of(m[0] - n0) : 1.f, a1 = n1 > m[1] ? exp2_of(m[1] - n1) : 1.f;
-            l[0] *= a0; l[1] *= a1;
+            if (!whole) {
 #pragma unroll
-            for (int x = 0; x < D / 8; ++x) { o[x][0] *= a0; o[x][1] *= a0; o[x][2] *= a1; o[x][3] *= a1; }
-            m[0] = n0; m[1] = n1;
-        }
-        // weights: exp2(s - m) carries 2^lv into the products and none of it into the sum
-        const float off0 = m[0] == -INFINITY ? 0.f : lvf - m[0], off1 = m[1] == -INFINITY ? 0.f : lvf - m[1];
-        float sum0 = 0.f, sum1 = 0.f;
-        uint32_t p[PIECES][2][4];
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 vs = *reinterpret_cast<const float2*>(scales + KEYS + 8 * j + 2 * quad);
-            const float f0 = vs.x * v_inverse * P_FACTOR, f1 = vs.y * v_inverse * P_FACTOR;   // at most 2^15
-            float w0 = exp2_of(c[j][0] + off0), w1 = exp2_of(c[j][1] + off0), w2 = exp2_of(c[j][2] + off1), w3 = exp2_of(c[j][3] + off1);
-            sum0 += w0 + w1;
-            sum1 += w2 + w3;
-            w0 *= f0; w1 *= f1; w2 *= f0; w3 *= f1;
-            if (!whole) {   // a hidden key's scale may be anything
-                if (c[j][0] == -INFINITY) w0 = 0.f;
-                if (c[j][1] == -INFINITY) w1 = 0.f;
-                if (c[j][2] == -INFINITY) w2 = 0.f;
-                if (c[j][3] == -INFINITY) w3 = 0.f;
+                    for (int e = 0; e < 2; ++e) {
+                        const int key = key0 + 8 * j + g;
+                        if (key > row_pos[nq][e] || (a.window > 0 && key <= row_pos[nq][e] - a.window) || key >= hi) c[nq][j >> 1][(j & 1) * 2 + e] = -INFINITY;
+                    }
             }
-            p[0][j >> 1][(j & 1) * 2] = pack_f16(w0, w1);
-            p[0][j >> 1][(j & 1) * 2 + 1] = pack_f16(w2, w3);
-            if constexpr (PIECES == 2) {
-                p[PIECES - 1][j >> 1][(j & 1) * 2] = pack_rest(w0, w1, p[0][j >> 1][(j & 1) * 2]);
-                p[PIECES - 1][j >> 1][(j & 1) * 2 + 1] = pack_rest(w2, w3, p[0][j >> 1][(j & 1) * 2 + 1]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) mx[e] = fmaxf(mx[e], c[nq][j >> 1][(j & 1) * 2 + e]);
+            bool raise = false;
+            float n[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
+                n[e] = fmaxf(m[nq][e], mx[e] + lvf);
+                raise |= n[e] > m[nq][e];
             }
+            if (__any_sync(0xffffffffu, raise)) {
+                const float a0 = n[0] > m[nq][0] ? exp2_of(m[nq][0] - n[0]) : 1.f, a1 = n[1] > m[nq][1] ? exp2_of(m[nq][1] - n[1]) : 1.f;
+                l[nq][0] *= a0; l[nq][1] *= a1;
+#pragma unroll
+                for (int x = 0; x < KSTEPS; ++x) { o[nq][x][0] *= a0; o[nq][x][1] *= a1; o[nq][x][2] *= a0; o[nq][x][3] *= a1; }
+                m[nq][0] = n[0]; m[nq][1] = n[1];
+            }
+            // weights: exp2(s - m) carries 2^lv into the products and none of it into the sum
+            float off[2], sum[2] = {0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 2; ++e) off[e] = m[nq][e] == -INFINITY ? 0.f : lvf - m[nq][e];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float& w = c[nq][j >> 1][(j & 1) * 2 + e];
+                    w = exp2_of(w + off[e]);
+                    sum[e] += w;
+                }
+            if (odd_scale) {   // a hidden key's scale may be anything
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float& w = c[nq][j >> 1][(j & 1) * 2 + e];
+                        w = w == 0.f ? 0.f : w * vf[j];
+                    }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) c[nq][j >> 1][(j & 1) * 2 + e] *= vf[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float w0 = c[nq][j >> 1][(j & 1) * 2], w1 = c[nq][j >> 1][(j & 1) * 2 + 1];
+                const uint32_t packed = pack_f16(w0, w1);
+                p[nq][0][j >> 1][j & 1] = transposed(packed);
+                if constexpr (PIECES == 2) p[nq][PIECES - 1][j >> 1][j & 1] = transposed(pack_rest(w0, w1, packed));
+            }
+            l[nq][0] += sum[0] * down;
+            l[nq][1] += sum[1] * down;
         }
-        const float down = exp2_of(-lvf);
-        l[0] += sum0 * down;
-        l[1] += sum1 * down;
 
-        // o += weights V. Lanes 0-7 / 8-15 of an ldmatrix name keys 16 s .. + 7 / 8 .. 15 at entries 16 n, lanes 16-31 the same keys 16 entries on
-        // (or, for an odd number of 16-entry columns, at the last one again).
-        const uint32_t v_addr = st + (KEYS + (lane & 15)) * PITCH;
+        // o += values x weights. Lanes 0-7 and 8-15 of an ldmatrix name keys 0-7 and 8-15 of a tile at 16-byte word n, lanes 16-31 the same keys at word
+        // n + 1 (or, for an odd number of words, at the last one again). Bytes of keys 2 quad and 2 quad + 1 at entries 2 g and 2 g + 1 come
+        // back: in another order they are the pairs of rows g and g + 8 of a left operand whose rows g are the even and g + 8 the odd entries.
+        const uint32_t v_row = (st + TENSOR_BYTES + (lane & 15) * PW) ^ row_swizzle(lane & 15);
         bool apart = false;
         if (!whole && tokens > 1) {   // a NaN among the values must not reach the rows that do not see it
             bool nan = false;
             for (int x = lane; x < KEYS * D / 4; x += 32) {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(smem + (st - smem_addr(smem)) + (KEYS + x / (D / 4)) * PITCH + x % (D / 4) * 4);
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(values + x * 4);
                 nan |= __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0;
             }
             apart = __any_sync(0xffffffffu, nan);
@@ -371,16 +609,16 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const Kv8Args a, c
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     uint32_t w[4];
-                    ldsm4_trans(w, v_addr + s * 16 * PITCH + (n + 1 < KSTEPS ? n + (lane >> 4) : n) * 16);
+                    ldsm4_trans(w, word_at(v_row ^ (SWIZZLED ? (lane >> 4) * 16 : 0), n) + s * 16 * PW + (!SWIZZLED && n + 1 < KSTEPS ? (lane >> 4) * 16 : 0));
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         if (n + half >= KSTEPS) break;
                         const uint32_t x = __byte_perm(w[2 * half], 0, 0x3120), z = __byte_perm(w[2 * half + 1], 0, 0x3120);
+                        const uint32_t vt[4] = {codes_to_f16(x), codes_to_f16_high(x), codes_to_f16(z), codes_to_f16_high(z)};
 #pragma unroll
-                        for (int pc = 0; pc < PIECES; ++pc) {
-                            mma_f16(o[2 * (n + half)], p[pc][s], codes_to_f16(x), codes_to_f16(z));
-                            mma_f16(o[2 * (n + half) + 1], p[pc][s], codes_to_f16(x >> 16), codes_to_f16(z >> 16));
-                        }
+                        for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                            for (int pc = 0; pc < PIECES; ++pc) mma_f16(o[nq][n + half], vt, p[nq][pc][s][0], p[nq][pc][s][1]);
                     }
                 }
             }
@@ -396,188 +634,189 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const Kv8Args a, c
                         const int key = key0 + 16 * s + 8 * e + 2 * quad;
                         keep[s][e] = (key <= pos && key >= from ? 0x00ff00ffu : 0u) | (key + 1 <= pos && key + 1 >= from ? 0xff00ff00u : 0u);
                     }
-                const bool take0 = row_pos[0] == pos, take1 = row_pos[1] == pos;
 #pragma unroll
                 for (int n = 0; n < KSTEPS; ++n) {
-                    float even[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        uint32_t w[4];
-                        ldsm4_trans(w, v_addr + s * 16 * PITCH + n * 16);
-                        const uint32_t x = __byte_perm(w[0], 0, 0x3120) & keep[s][0], z = __byte_perm(w[1], 0, 0x3120) & keep[s][1];
+                    for (int nq = 0; nq < NQ; ++nq) {
+                        float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int pc = 0; pc < PIECES; ++pc) {
-                            mma_f16(even, p[pc][s], codes_to_f16(x), codes_to_f16(z));
-                            mma_f16(odd, p[pc][s], codes_to_f16(x >> 16), codes_to_f16(z >> 16));
+                        for (int s = 0; s < 2; ++s) {
+                            uint32_t w[4];
+                            ldsm4_trans(w, word_at(v_row, n) + s * 16 * PW);
+                            const uint32_t x = __byte_perm(w[0], 0, 0x3120) & keep[s][0], z = __byte_perm(w[1], 0, 0x3120) & keep[s][1];
+                            const uint32_t vt[4] = {codes_to_f16(x), codes_to_f16_high(x), codes_to_f16(z), codes_to_f16_high(z)};
+#pragma unroll
+                            for (int pc = 0; pc < PIECES; ++pc) mma_f16(sum, vt, p[nq][pc][s][0], p[nq][pc][s][1]);
                         }
-                    }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (e < 2 ? take0 : take1) { o[2 * n][e] += even[e]; o[2 * n + 1][e] += odd[e]; }
+                        for (int e = 0; e < 4; ++e)
+                            if (row_pos[nq][e & 1] == pos) o[nq][n][e] += sum[e];
+                    }
                 }
             }
         }
-        __syncwarp();   // every lane has read the stage before the next turn fills it
+        fence_proxy_async();   // every lane has read the stage before the next turn's copies fill it
+        __syncwarp();
     }
-    cp_async_wait<0>();
+    turn += mine;
 
-    // ---- join: warps in shared memory, then blocks of the cluster
-    l[0] += __shfl_xor_sync(0xffffffffu, l[0], 1);
-    l[1] += __shfl_xor_sync(0xffffffffu, l[1], 1);
-    l[0] += __shfl_xor_sync(0xffffffffu, l[0], 2);
-    l[1] += __shfl_xor_sync(0xffffffffu, l[1], 2);
-    __syncwarp();
-    float* part = reinterpret_cast<float*>(smem + (size_t)warp * STAGES * STAGE_BYTES);   // [ROWS][D]
-#pragma unroll
-    for (int n = 0; n < KSTEPS; ++n) {
-        if (g < rows) *reinterpret_cast<float4*>(part + g * D + 16 * n + 4 * quad) = make_float4(o[2 * n][0], o[2 * n + 1][0], o[2 * n][1], o[2 * n + 1][1]);
-        if (g + 8 < rows) *reinterpret_cast<float4*>(part + (g + 8) * D + 16 * n + 4 * quad) = make_float4(o[2 * n][2], o[2 * n + 1][2], o[2 * n][3], o[2 * n + 1][3]);
-    }
-    if (quad == 0) {
-        warp_ml[warp * ROWS + g] = make_float2(m[0], l[0]);
-        warp_ml[warp * ROWS + g + 8] = make_float2(m[1], l[1]);
-    }
-    __syncthreads();
+    // ---- the tile's result, or what this warp has of it
+    const bool whole_tile = at.block == 0 && count == at.of.blocks;
+    if (at.block == 0 && !whole_tile)
+        cut = {(item - count + at.of.blocks - 1) / share, q_begin + tok0, kvh * G + hg * a.heads_per_tile, rows, min(a.heads_per_tile, G - hg * a.heads_per_tile), base_exp, {0, 0}};
     const float unscale = exp2_of((float)base_exp);
-    auto put = [&](int r, int d, float4 v, float total) {
-        const int tok = r / a.heads_per_tile, head = hg * a.heads_per_tile + r % a.heads_per_tile;
-        if (head >= G) return;
-        const float f = (1.f / P_FACTOR) / total;
-        v.x = v.x * f * unscale; v.y = v.y * f * unscale; v.z = v.z * f * unscale; v.w = v.w * f * unscale;
-        if (total == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-        store4(out + ((size_t)(t.q_begin + tok0 + tok) * a.H + (size_t)kvh * G + head) * D + d, v);
-    };
-    for (int x = threadIdx.x; x < rows * (D / 4); x += THREADS) {
-        const int r = x / (D / 4), d = x % (D / 4) * 4;
-        float top = -INFINITY;
+    const size_t place = (size_t)2 * me + (at.block == 0 ? 1 : 0);
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, warp_ml[w * ROWS + r].x);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        float total = 0.f;
+    for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const float2 ml = warp_ml[w * ROWS + r];
-            const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_of(ml.x - top);   // (a NaN sum without a maximum is kept)
-            const float4 u = *reinterpret_cast<const float4*>(smem + (size_t)w * STAGES * STAGE_BYTES + (size_t)(r * D + d) * 4);
-            if (f != 0.f) { v.x += u.x * f; v.y += u.y * f; v.z += u.z * f; v.w += u.w * f; total += ml.y * f; }
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) l[nq][e] += __shfl_xor_sync(0xffffffffu, l[nq][e], x);
+            const int r = 8 * nq + 2 * quad + e, tok = r / a.heads_per_tile, head = hg * a.heads_per_tile + r % a.heads_per_tile;
+            if (r >= rows || head >= G) continue;
+            const float total = l[nq][e];
+            if (whole_tile) {
+                const float f = (1.f / P_FACTOR) / total;
+                T* row = out + ((size_t)(q_begin + tok0 + tok) * a.H + (size_t)kvh * G + head) * D + 2 * g;
+#pragma unroll
+                for (int n = 0; n < KSTEPS; ++n)
+                    store2(row + 16 * n, total == 0.f ? make_float2(0.f, 0.f) : make_float2(o[nq][n][e] * f * unscale, o[nq][n][2 + e] * f * unscale));
+            } else {
+                // (all pieces of a tile are relative to the same scale)
+                if (g == 0) left.ml[place * ROWS + r] = make_float2(m[nq][e], total);
+                float* row = left.sums + (place * ROWS + r) * D + 2 * g;
+#pragma unroll
+                for (int n = 0; n < KSTEPS; ++n) *reinterpret_cast<float2*>(row + 16 * n) = make_float2(o[nq][n][e], o[nq][n][2 + e]);
+            }
         }
-        if (splits == 1) {
-            put(r, d, v, total);
-        } else {   // over the first warp's part: this thread alone has read these entries of it
-            *reinterpret_cast<float4*>(smem + (size_t)(r * D + d) * 4) = v;
-            if (d == 0) block_ml[r] = make_float2(top, total);
-        }
+    __syncwarp();
     }
-    if (splits == 1) return;
-    cluster_barrier();
-    const int pieces = rows * (D / 4);
-    for (int x = rank * THREADS + threadIdx.x; x < pieces; x += splits * THREADS) {
-        const int r = x / (D / 4), d = x % (D / 4) * 4;
-        const uint32_t ml_at = smem_addr(block_ml + r), v_at = smem_addr(smem) + (uint32_t)(r * D + d) * 4;
-        float top = -INFINITY;
-        for (int s = 0; s < splits; ++s) top = fmaxf(top, ld_cluster_f2(map_to_rank(ml_at, s)).x);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        float total = 0.f;
-        for (int s = 0; s < splits; ++s) {
-            const float2 ml = ld_cluster_f2(map_to_rank(ml_at, s));
-            const float4 u = ld_cluster_f4(map_to_rank(v_at, s));
-            const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_of(ml.x - top);
-            if (f != 0.f) { v.x += u.x * f; v.y += u.y * f; v.z += u.z * f; v.w += u.w * f; total += ml.y * f; }
-        }
-        put(r, d, v, total);
-    }
-    cluster_barrier();   // no block leaves while another may still read its shared memory
+    if (lane == 0) left.cuts[me] = cut;
 }
 
-template <typename T>
-int launch(void* out, const void* q, const Kv8Args& a, int tiles, int splits, cudaStream_t stream) {
-    constexpr size_t smem = smem_bytes<sizeof(T) == 4 ? 2 : 1>();
-    static_assert(smem <= 227 * 1024, "shared memory of a block");
-    auto kernel = attn_kv8_kernel<T>;
-    const long long grid = (long long)tiles * a.KV * a.head_groups * splits;
-    if (grid > 0x7fffffffll) return OXR_BAD_ARGUMENT;
+// Joins the pieces of the tiles that lie in more than one warp's stretch. Block b takes the tile that stretch b ends in, if it began there. A
+// thread has four entries of a row; where the rows leave threads over, they take the pieces in turn.
+constexpr int JOIN_THREADS = 256;
+template <typename T, int NQ>
+__global__ void __launch_bounds__(JOIN_THREADS) attn_kv8_join_kernel(T* __restrict__ out, const Pieces left, const int H, const int heads_per_tile) {
+    constexpr int ROWS = 8 * NQ, WORDS = D / 4;
+    __shared__ float4 sums[JOIN_THREADS];
+    __shared__ float2 ml[JOIN_THREADS];
+    pdl_wait();
+    pdl_trigger();
+    const int first = blockIdx.x;
+    const int4 c0 = __ldcg(reinterpret_cast<const int4*>(left.cuts + first)), c1 = __ldcg(reinterpret_cast<const int4*>(left.cuts + first) + 1);
+    const Cut cut = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, {0, 0}};
+    if (cut.last < 0) return;
+    const float unscale = exp2_of((float)cut.base_exp);
+    const int all = cut.rows * WORDS;
+    int ways = 1;      // threads that share an entry's pieces
+    while (ways * 2 * all <= JOIN_THREADS) ways *= 2;
+    for (int x0 = 0; x0 < all; x0 += JOIN_THREADS) {
+        const int x = ways > 1 ? threadIdx.x % all : x0 + threadIdx.x, way = ways > 1 ? threadIdx.x / all : 0;
+        const int r = x / WORDS, d = x % WORDS * 4;
+        const bool there = x < all && way < ways;
+        float top = -INFINITY, total = 0.f;
+        float4 v[1] = {make_float4(0.f, 0.f, 0.f, 0.f)};
+        if (there) {
+            for (int w0 = first + way; w0 <= cut.last; w0 += 8 * ways) {     // eight pieces at a time
+                float2 y[8];
+                float4 u[8][1];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int w = w0 + k * ways;
+                    const size_t at = ((size_t)2 * w + (w == first ? 1 : 0)) * ROWS + r;
+                    y[k] = w <= cut.last ? __ldcg(left.ml + at) : make_float2(-INFINITY, 0.f);
+                    u[k][0] = w <= cut.last ? __ldcg(reinterpret_cast<const float4*>(left.sums + at * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) add_piece<1>(top, total, v, y[k], u[k]);
+            }
+        }
+        if (ways > 1) {
+            sums[threadIdx.x] = v[0];
+            ml[threadIdx.x] = make_float2(top, total);
+            __syncthreads();
+            if (there && way == 0)
+                for (int k = 1; k < ways; ++k) {
+                    const float4 u[1] = {sums[k * all + x]};
+                    add_piece<1>(top, total, v, ml[k * all + x], u);
+                }
+        }
+        const int head = r % heads_per_tile;
+        if (there && way == 0 && head < cut.heads) {
+            const float f = (1.f / P_FACTOR) / total;
+            float4 z = make_float4(v[0].x * f * unscale, v[0].y * f * unscale, v[0].z * f * unscale, v[0].w * f * unscale);
+            if (total == 0.f) z = make_float4(0.f, 0.f, 0.f, 0.f);
+            store4(out + ((size_t)(cut.token + r / heads_per_tile) * H + cut.head + head) * D + d, z);
+        }
+    }
+}
+
+// A pool of pages seen as boxes of `piece` keys x PW bytes of one KV head.
+bool make_map(CUtensorMap* map, const void* base, const Kv8Args& a, int piece) {
+    OxrEncodeTiledFn fn = oxr_encode_tiled();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)a.KV * D, (cuuint64_t)a.page_size, (cuuint64_t)a.num_pages};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.KV * D, (cuuint64_t)a.page_stride};
+    const cuuint32_t box[3] = {(cuuint32_t)PW, (cuuint32_t)piece, 1u};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    const CUtensorMapSwizzle swizzle = !SWIZZLED ? CU_TENSOR_MAP_SWIZZLE_NONE : PW == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : PW == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, bool TMA, int NQ>
+int allow() {   // once per device and thread: the shared memory of the kernel
     static thread_local int ready = -1;
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess) return oxr_launch_status();
-    if (ready != device) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return oxr_launch_status();
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return oxr_launch_status();
-        ready = device;
-    }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attrs[2];
-    int n = 0;
-    if (splits > 1) {
-        attrs[n].id = cudaLaunchAttributeClusterDimension;
-        attrs[n].val.clusterDim.x = (unsigned)splits;
-        attrs[n].val.clusterDim.y = 1;
-        attrs[n].val.clusterDim.z = 1;
-        ++n;
-    }
-    if (oxr_chain_kernels) {
-        attrs[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attrs[n].val.programmaticStreamSerializationAllowed = 1;
-        ++n;
-    }
-    cfg.attrs = attrs;
-    cfg.numAttrs = n;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, (T*)out, (const T*)q, a, splits);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        return 1000 + (int)e;
-    }
+    if (ready == device) return 0;
+    if (cudaFuncSetAttribute(attn_kv8_kernel<T, TMA, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<T, NQ>::SMEM) != cudaSuccess) return oxr_launch_status();
+    ready = device;
     return 0;
 }
 
-template <typename T>
-int clusters_of(int splits) {
-    constexpr size_t smem = smem_bytes<sizeof(T) == 4 ? 2 : 1>();
-    auto kernel = attn_kv8_kernel<T>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
-        cudaGetLastError();
-        return 0;
-    }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)splits);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)splits;
-    attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
-        cudaGetLastError();
-        return 0;
-    }
-    return n;
+template <typename T, int NQ>
+int launch(void* out, const void* q, const Kv8Args& a, int blocks, float* scratch, cudaStream_t stream) {
+    int piece_shift = 0;
+    while (piece_shift < 5 && a.page_size % (2 << piece_shift) == 0) ++piece_shift;
+    CUtensorMap map_k = {}, map_v = {};
+    const bool tma = piece_shift >= 3 && a.num_pages > 0 && make_map(&map_k, a.k_cache, a, 1 << piece_shift) && make_map(&map_v, a.v_cache, a, 1 << piece_shift);
+    const int code = tma ? allow<T, true, NQ>() : allow<T, false, NQ>();
+    if (code != 0) return code;
+    const int warps = blocks * WARPS;
+    float2* ml = reinterpret_cast<float2*>(scratch + (size_t)2 * warps * 8 * NQ * D);
+    const Pieces left = {scratch, ml, reinterpret_cast<Cut*>(ml + (size_t)2 * warps * 8 * NQ)};
+    const dim3 grid(blocks), threads(THREADS);
+    if (tma) oxr_launch(attn_kv8_kernel<T, true, NQ>, grid, threads, Shape<T, NQ>::SMEM, stream, true, (T*)out, (const T*)q, map_k, map_v, piece_shift, a, left);
+    else oxr_launch(attn_kv8_kernel<T, false, NQ>, grid, threads, Shape<T, NQ>::SMEM, stream, true, (T*)out, (const T*)q, map_k, map_v, piece_shift, a, left);
+    if (warps > 1) oxr_launch(attn_kv8_join_kernel<T, NQ>, dim3(warps - 1), dim3(JOIN_THREADS), 0, stream, true, (T*)out, left, a.H, a.heads_per_tile);
+    return oxr_launch_status();
 }
 }  // namespace
 
 OXR_API void oxr_set_chain(int on) { oxr_chain_kernels = on; }
 OXR_API int oxr_kv8_head_dim() { return D; }
-// How many clusters of `splits` blocks the current device holds at a time (0: none can be launched).
-OXR_API int oxr_kv8_clusters(int dtype, int splits) { return dtype == 0 ? clusters_of<float>(splits) : clusters_of<__nv_bfloat16>(splits); }
+// Blocks (of four warps) of the split-key kernel that an SM holds.
+OXR_API int oxr_kv8_blocks_per_sm(int dtype, int tile_rows) {
+    return tile_rows == 8 ? (dtype == 0 ? Shape<float, 1>::BLOCKS : Shape<__nv_bfloat16, 1>::BLOCKS) : (dtype == 0 ? Shape<float, 2>::BLOCKS : Shape<__nv_bfloat16, 2>::BLOCKS);
+}
 
 // q [n_tokens, H, D] (tokens q_stride entries apart), out [n_tokens, H, D]; K and V pools of e4m3 codes with pages page_stride bytes apart and each
 // page [page_size, KV, D]; scales [num_pages, KV]; cu_q [n + 1], ctx_lens [n], block_table [n, table_width]. Requests of min_q .. max_q new
-// tokens are worked on; `any_q` is the most that any request may bring. dtype 0: fp32, 1: bf16.
+// tokens are worked on; `any_q` is the most that any request may bring. dtype 0: fp32, 1: bf16; tiles of `tile_rows` (8 or 16) rows. `blocks` of four warps share
+// the work; `scratch` holds 8 * blocks * tile_rows * (D + 2) + 32 * blocks words.
 OXR_API int oxr_kv8_attention(void* out, const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, const int* cu_q,
                               const int* ctx_lens, const int* block_table, int n, int n_tokens, int table_width, int page_size, long long page_stride,
-                              int num_pages, int H, int KV, long long q_stride, float scale, int window, int min_q, int max_q, int any_q, int tiles, int splits,
-                              int dtype, int* status, cudaStream_t stream) {
-    if (n < 0 || n_tokens < 0 || KV <= 0 || H <= 0 || H % KV || page_size <= 0 || table_width < 0 || num_pages < 0 || window < 0 || tiles < 0) return OXR_BAD_ARGUMENT;
-    if (splits < 1 || splits > 16 || (splits & (splits - 1)) || (dtype != 0 && dtype != 1) || any_q < 1 || min_q < 1) return OXR_BAD_ARGUMENT;
-    if (tiles == 0 || n == 0 || n_tokens == 0) return 0;
-    Kv8Args a = kv8_args(k_cache, v_cache, k_scale, v_scale, cu_q, ctx_lens, block_table, n, n_tokens, table_width, page_size, page_stride, num_pages, H, KV,
-                         q_stride, scale, window, min_q, max_q, any_q, ROWS, status);
-    return dtype == 0 ? launch<float>(out, q, a, tiles, splits, stream) : launch<__nv_bfloat16>(out, q, a, tiles, splits, stream);
+                              int num_pages, int H, int KV, long long q_stride, float scale, int window, int min_q, int max_q, int any_q, int tile_rows, int blocks,
+                              float* scratch, int dtype, int* status, cudaStream_t stream) {
+    if (n < 0 || n_tokens < 0 || KV <= 0 || H <= 0 || H % KV || page_size <= 0 || table_width < 0 || num_pages < 0 || window < 0) return OXR_BAD_ARGUMENT;
+    if (blocks < 1 || blocks > 65536 || scratch == nullptr || (dtype != 0 && dtype != 1) || any_q < 1 || min_q < 1 || (tile_rows != 8 && tile_rows != 16))
+        return OXR_BAD_ARGUMENT;
+    if (n == 0 || n_tokens == 0) return 0;
+    const Kv8Args a = kv8_args(k_cache, v_cache, k_scale, v_scale, cu_q, ctx_lens, block_table, n, n_tokens, table_width, page_size, page_stride, num_pages, H,
+                               KV, q_stride, scale, window, min_q, max_q, any_q, tile_rows, status);
+    if (tile_rows == 8) return dtype == 0 ? launch<float, 1>(out, q, a, blocks, scratch, stream) : launch<__nv_bfloat16, 1>(out, q, a, blocks, scratch, stream);
+    return dtype == 0 ? launch<float, 2>(out, q, a, blocks, scratch, stream) : launch<__nv_bfloat16, 2>(out, q, a, blocks, scratch, stream);
 }

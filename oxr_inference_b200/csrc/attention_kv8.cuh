@@ -123,10 +123,15 @@ __device__ __forceinline__ Kv8Tile kv8_find_tile(const Kv8Args& a, int index, in
     return t;
 }
 
-// Two e4m3 codes (the low 16 bits) as two fp16 numbers: exact, NaN stays NaN.
+// Two e4m3 codes (the low or the high 16 bits) as two fp16 numbers: exact, NaN stays NaN.
 __device__ __forceinline__ uint32_t codes_to_f16(uint32_t w) {
     uint32_t r;
     asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(w));
+    return r;
+}
+__device__ __forceinline__ uint32_t codes_to_f16_high(uint32_t w) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(w));
     return r;
 }
 // The integer e with 2^(e - 1) < s <= 2^e for a positive finite s (subnormal ones count as 2^-126).

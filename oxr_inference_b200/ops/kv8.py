@@ -19,9 +19,6 @@ from oxr_inference_b200.ops import build
 from oxr_inference_b200.ops.build import BuildError
 
 KV8_DTYPE = torch.float8_e4m3fn
-KV8_ROWS = 16
-"""Rows (token, query head of one KV head) of a tile of the split-key kernel."""
-KV8_MAX_SPLITS = 16
 _INT = torch.int32
 
 _kv8: dict = {}
@@ -33,10 +30,10 @@ def _kv8_lib(head_dim: int):
     if lib is None:
         lib = build.kv8_library(head_dim)
         p, i, f, ll = c_void_p, c_int, c_float, c_longlong
-        lib.oxr_kv8_attention.argtypes = [p] * 9 + [i, i, i, i, ll, i, i, i, ll, f, i, i, i, i, i, i, i, p, p]
+        lib.oxr_kv8_attention.argtypes = [p] * 9 + [i, i, i, i, ll, i, i, i, ll, f, i, i, i, i, i, i, p, i, p, p]
         lib.oxr_kv8_attention.restype = c_int
-        lib.oxr_kv8_clusters.argtypes = [i, i]
-        lib.oxr_kv8_clusters.restype = c_int
+        lib.oxr_kv8_blocks_per_sm.argtypes = [i, i]
+        lib.oxr_kv8_blocks_per_sm.restype = c_int
         lib.oxr_kv8_head_dim.restype = c_int
         if lib.oxr_kv8_head_dim() != head_dim:
             raise BuildError(f"library for head size {head_dim} reports {lib.oxr_kv8_head_dim()}")
@@ -133,25 +130,15 @@ def store_kv8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: to
 
 
 @functools.lru_cache(maxsize=None)
-def _kv8_cluster_room(head_dim: int, code: int, device: int) -> tuple[tuple[int, int], ...]:
-    """(blocks of a cluster, clusters that the device holds at a time) for every size that can be launched."""
-    lib = _kv8_lib(head_dim)
-    room = [(s, lib.oxr_kv8_clusters(code, s)) for s in (1, 2, 4, 8, 16)]
-    return tuple((s, c) for s, c in room if c > 0)
+def _kv8_room(head_dim: int, code: int, tile_rows: int) -> int:
+    """Blocks of the split-key kernel that the current device holds at a time."""
+    return ops.num_sms() * _kv8_lib(head_dim).oxr_kv8_blocks_per_sm(code, tile_rows)
 
 
-def kv8_splits(units: int, key_blocks: int, room: tuple[tuple[int, int], ...]) -> int:
-    """Blocks (of four warps) that share the keys of each of ``units`` tiles, the longest of ``key_blocks`` blocks of 32 keys: the size with the least
-    waves x (a block's own cost + key blocks per warp), the smaller among equals. A block costs about as much before its first keys arrive and
-    after its last as eight key blocks of a warp."""
-    best, best_cost = 1, None
-    for splits, clusters in room:
-        if splits > 1 and splits * 4 > key_blocks:
-            break
-        cost = -(-units // clusters) * (8 + -(-key_blocks // (splits * 4)))
-        if best_cost is None or cost < best_cost:
-            best, best_cost = splits, cost
-    return best
+def kv8_blocks(tiles: int, key_blocks: int, room: int) -> int:
+    """Blocks of four warps among which a step's work is dealt out: as many as the device holds at a time, fewer where a warp would get
+    less than one block of 32 keys (``tiles`` tiles of at most ``key_blocks`` of them)."""
+    return max(1, min(room, -(-tiles * key_blocks // 4)))
 
 
 def paged_attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, *,
@@ -187,15 +174,18 @@ def paged_attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         return out
     lib = _kv8_lib(d)
     group = heads // kv
-    heads_per_tile = min(group, KV8_ROWS)
-    per_tile = KV8_ROWS // heads_per_tile
-    tiles = n if max_q_len == 1 else min(tokens, n * -(-max_q_len // per_tile), n + tokens // per_tile)
-    seen = min(kv_len_bound, window + max_q_len) if window > 0 else kv_len_bound
-    splits = kv8_splits(tiles * kv * -(-group // heads_per_tile), -(-max(seen, 1) // 32), _kv8_cluster_room(d, code, device))
+    rows = 8 if group * max_q_len <= 8 else 16      # the split-key kernel's tiles: (token, query head) pairs of one KV head
+    heads_per_tile = min(group, rows)
+    per_tile = rows // heads_per_tile
+    tiles = min(tokens, n * -(-max_q_len // per_tile), n + tokens // per_tile) * kv * -(-group // heads_per_tile)
+    seen = min(kv_len_bound, window + max_q_len + 32) if window > 0 else kv_len_bound
+    blocks = kv8_blocks(tiles, max(1, -(-seen // 32)), _kv8_room(d, code, rows))
+    scratch = torch.empty(8 * blocks * rows * (d + 2) + 32 * blocks, dtype=torch.float32, device=q.device)
     ops._done(lib.oxr_kv8_attention(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                     cu_q.data_ptr(), ctx_lens.data_ptr(), block_table.data_ptr(), n, tokens, block_table.shape[1], page, page_stride, pages,
-                                    heads, kv, q_stride, float(scale), int(window), 1, int(max_q_len), int(max_q_len), tiles, splits, code,
+                                    heads, kv, q_stride, float(scale), int(window), 1, int(max_q_len), int(max_q_len), rows, blocks, scratch.data_ptr(), code,
                                     status.data_ptr(), ops._stream()), "paged_attention_kv8")
+    ops.launch_count += 1
     return out
 
 
