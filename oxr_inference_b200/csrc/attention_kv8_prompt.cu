@@ -1,0 +1,546 @@
+// Attention of long portions of prompts over the 8-bit paged cache on tcgen05, for bf16 queries and head sizes up to 128. Compiled once per head size.
+//
+// The formula is that of attention_kv8.cu, and so are the tricks with the scales. A tile is 256 rows, (token, query head) pairs of one KV head, in two
+// halves of 128 (a row is a lane of tensor memory). Per block of 128 keys and half
+//     S = Q K^T      tcgen05.mma on fp16 operands in shared memory, fp32 sums in tensor memory;
+//     softmax        a thread per row: P = exp2(S - m), fp16, back into tensor memory over the columns that S came from;
+//     O += P V       tcgen05.mma with P from tensor memory.
+// kind::f8f6f4 would take the codes as they are, but its other operand would have to have 8 bits too, and two e4m3 numbers for each weight cost the
+// softmax threads more than what is done instead: seven warps turn the codes of a block, while it passes from global to shared memory, into fp16
+// numbers, times the ratio of their page's scale to the block's largest (a power of two when the scales are; the products are then exact). The block's
+// largest key scale goes into the factor of the scores, the largest value scale as its logarithm into the exponent of the weights, so that
+// neither costs the softmax an instruction per key. Weights are kept as 2^7 P against a maximum that is raised in steps of 2^8: below 2^15 in
+// fp16, with their eleven bits down to 2^-21 of the largest.
+// Warps: 0 issues the products and owns the tensor memory, 1 to 3 and 12 to 15 bring in keys and values, 4 to 7 and 8 to 11 are the
+// softmax of the first and the second half; setmaxnreg gives those 160 registers (128 scores and what goes with them) and the others 96 (with 64 the
+// codes on their way were spilled: 404 us instead of 146, see the launcher).
+// What bounds it: see the launcher. Every wait on an mbarrier is bounded.
+#include <cuda_fp16.h>
+
+#include "tma.cuh"
+
+#ifndef HEAD_DIM
+#error "compile with -DHEAD_DIM=<head size>"
+#endif
+
+#include "attention_kv8.cuh"
+
+#if HEAD_DIM <= 128
+namespace {
+constexpr int HALF_ROWS = 128, TILE_ROWS = 2 * HALF_ROWS, KEYS = 128, STAGES = 2;
+constexpr int THREADS = 512, LOADERS = 224;
+constexpr int PANELS = (D + 63) / 64;                    // of 64 entries: 128 bytes a row, 128-byte swizzle
+constexpr int PANEL_BYTES = 128 * 128;
+constexpr int TENSOR_BYTES = PANELS * PANEL_BYTES;       // a half's queries, a block's keys, a block's values
+constexpr int O_COLS = PANELS * 64;                      // whole panels: what the columns behind D hold is not looked at
+constexpr int WORDS = D / 16;                            // 16 codes of a key: what a loader thread takes at a time
+constexpr int PASSES = (KEYS * WORDS + LOADERS - 1) / LOADERS;
+constexpr int INFO = 4;                                  // blocks whose pages and scales are at hand
+constexpr float RAISE = 8.f;
+constexpr float P_SHIFT = 7.f;
+constexpr uint32_t TMEM_COLS = 512;                      // S | P of half h at 128 h, O of half h at 256 + h O_COLS
+
+struct BlockInfo {
+    long long row[KEYS];       // byte offset of each key's row in the pools; -1: zeros stand for it
+    float k_scale[KEYS], v_scale[KEYS];
+    float k_most[4], v_most[4];   // of each 32 keys: the largest scale
+    float factor, shift;       // of the block: its largest key scale; log2 of its largest value scale, relative to the last page's
+};
+struct Shared {
+    BlockInfo info[INFO];
+    uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_full[2], o_done[2], q_ready;
+    uint32_t tmem;
+    int nan_values;            // a block that not every row sees in full has a NaN among its values
+};
+constexpr size_t SMEM = (2 + 2 * STAGES) * (size_t)TENSOR_BYTES + sizeof(Shared);
+static_assert(SMEM <= 227 * 1024, "shared memory of a block");
+
+__device__ __forceinline__ uint64_t desc_kmajor(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// rows are keys (the products' depth), 64 entries in 128 bytes; the next 64 entries a panel on
+__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(PANEL_BYTES >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// kind::f16, fp32 sums, both operands fp16, A K-major, B K-major or MN-major
+__host__ __device__ constexpr uint32_t idesc_of(int m, int n, bool b_mn_major) {
+    return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+                 ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+                 ::"r"(d), "r"(ta), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+#define KV8_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define KV8_I8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t (&r)[32]) {   // tcgen05.wait::ld has to follow
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : KV8_R8(r, 0), KV8_R8(r, 8), KV8_R8(r, 16), KV8_R8(r, 24) : "r"(taddr));
+}
+__device__ __forceinline__ void ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : KV8_R8(r, 0), KV8_R8(r, 8) : "r"(taddr));
+}
+__device__ __forceinline__ void st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), KV8_I8(r, 0), KV8_I8(r, 8) : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ bool one_lane() {
+    uint32_t pred;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
+    return pred != 0;
+}
+// Two fp32 numbers in a pair of registers, for the packed fp32 instructions.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ void loaders_meet() { asm volatile("bar.sync 1, %0;" ::"n"(LOADERS) : "memory"); }
+__device__ __forceinline__ bool has_nan(uint4 w) {
+    constexpr uint32_t M = 0x7f7f7f7fu;
+    return (__vcmpeq4(w.x & M, M) | __vcmpeq4(w.y & M, M) | __vcmpeq4(w.z & M, M) | __vcmpeq4(w.w & M, M)) != 0;
+}
+__device__ __forceinline__ float usable(float scale) { return scale > 0.f && scale < INFINITY ? scale : 0.f; }
+
+__global__ void __launch_bounds__(THREADS, 1)
+attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ q, const Kv8Args a, const int tiles) {
+    extern __shared__ __align__(1024) unsigned char smem[];     // nothing static stands before it
+    unsigned char* q_tiles = smem;                              // [half] queries
+    unsigned char* k_ring = q_tiles + 2 * TENSOR_BYTES;         // [STAGES]
+    unsigned char* v_ring = k_ring + STAGES * TENSOR_BYTES;
+    Shared& sh = *reinterpret_cast<Shared*>(v_ring + STAGES * TENSOR_BYTES);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_wait();
+    pdl_trigger();
+
+    // later tiles of a prompt see more keys: the long ones first, the heads of a tile side by side
+    const int per_tile = a.KV * a.head_groups, y = (int)(blockIdx.x % (unsigned)per_tile);
+    const int kvh = y / a.head_groups, hg = y % a.head_groups, G = a.H / a.KV;
+    const Kv8Tile t = kv8_find_tile(a, tiles - 1 - (int)(blockIdx.x / (unsigned)per_tile), a.tokens_per_tile, blockIdx.x == 0);
+    if (t.req < 0) return;
+    const int tokens = min(a.tokens_per_tile, t.q_len - t.tok0), rows = tokens * a.heads_per_tile;
+    const int first_pos = __ldg(a.ctx_lens + t.req) - t.q_len + t.tok0, last_pos = first_pos + tokens - 1;
+    int hi = last_pos + 1;
+    const int lo = a.window > 0 ? max(0, first_pos - a.window + 1) : 0;
+    if (hi > (long long)a.table_width * a.page_size) {
+        if (threadIdx.x == 0) oxr_report(a.status, OXR_BAD_PAGE, t.req);
+        hi = a.table_width * a.page_size;
+    }
+    const int block0 = lo / KEYS, count = hi > lo ? (hi + KEYS - 1) / KEYS - block0 : 0;
+    const bool half1_live = rows > HALF_ROWS;
+    const int* table_row = a.block_table + (size_t)t.req * a.table_width;
+    const int last_lo = a.window > 0 ? last_pos - a.window + 1 : 0;
+    auto partial = [&](int b) { return (block0 + b) * KEYS < last_lo || (block0 + b) * KEYS + KEYS - 1 > first_pos; };   // not every row sees all of it
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) { mbar_init(sh.k_full + i, LOADERS / 32); mbar_init(sh.k_empty + i, 1); mbar_init(sh.v_full + i, LOADERS / 32); mbar_init(sh.v_empty + i, 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(sh.s_full + i, 1); mbar_init(sh.p_full + i, 4); mbar_init(sh.o_done + i, 1); }
+        mbar_init(&sh.q_ready, 8);
+        mbar_fence_init();
+        sh.nan_values = 0;
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sh.tmem)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sh.tmem;
+    int base_exp = 0;       // what value scales are relative to: the last visible page's
+    if (count > 0) {
+        const int page = __ldg(table_row + a.page_of(hi - 1));
+        if (page >= 0 && page < a.num_pages) {
+            const float s = usable(__ldg(a.v_scale + (size_t)page * a.KV + kvh));
+            if (s > 0.f) base_exp = scale_exponent(s);
+        }
+    }
+
+    if (warp < 4 || warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        if (warp > 0) {
+            // ------------------------------------------------------------------ keys and values come in
+            const int lt = warp < 4 ? threadIdx.x - 32 : threadIdx.x - 12 * 32 + 96;      // 0 .. 223
+            // The first 128 threads look after a key of a block each: its page two blocks ahead, its scales one block ahead.
+            auto page_for = [&](int b) -> int {        // -1: none to be read
+                const int key = (block0 + b) * KEYS + lt;
+                if (lt >= KEYS || b >= count || key < lo || key >= hi) return -1;
+                const int page = __ldg(table_row + a.page_of(key));
+                if (page >= 0 && page < a.num_pages) return page;
+                oxr_report(a.status, OXR_BAD_PAGE, t.req);
+                return -1;
+            };
+            auto put_info = [&](int b, int page, float ks, float vs) {
+                if (lt >= KEYS) return;
+                BlockInfo& f = sh.info[b % INFO];
+                const int key = (block0 + b) * KEYS + lt;
+                f.row[lt] = page >= 0 ? (long long)page * a.page_stride + (a.in_page(key) * a.KV + kvh) * D : -1;
+                f.k_scale[lt] = ks;
+                f.v_scale[lt] = vs;
+                // (positive floats compare as integers do)
+                const uint32_t km = __reduce_max_sync(0xffffffffu, __float_as_uint(usable(ks))), vm = __reduce_max_sync(0xffffffffu, __float_as_uint(usable(vs)));
+                if (lane == 0) { f.k_most[lt / 32] = __uint_as_float(km); f.v_most[lt / 32] = __uint_as_float(vm); }
+            };
+            auto scale_of = [&](const float* scales, int page) { return page >= 0 ? __ldg(scales + (size_t)page * a.KV + kvh) : 0.f; };
+            // Which 16 codes a thread takes in each pass: mostly the same columns of a key so many further on.
+            constexpr bool SAME_COLUMNS = LOADERS % WORDS == 0;
+            const int first_key = lt / WORDS, first_col = lt % WORDS;
+            auto key_of = [&](int p) { return SAME_COLUMNS ? first_key + p * (LOADERS / WORDS) : (lt + p * LOADERS) / WORDS; };
+            auto col_of = [&](int p) { return SAME_COLUMNS ? first_col : (lt + p * LOADERS) % WORDS; };
+            uint4 kc[PASSES], vc[PASSES];
+            auto ask = [&](uint4 (&c)[PASSES], const unsigned char* pool, int b) {
+                if (b >= count) return;
+                const BlockInfo& f = sh.info[b % INFO];
+#pragma unroll
+                for (int p = 0; p < PASSES; ++p) {
+                    const long long row = key_of(p) < KEYS ? f.row[key_of(p)] : -1;
+                    c[p] = row >= 0 ? __ldg(reinterpret_cast<const uint4*>(pool + row + col_of(p) * 16)) : make_uint4(0, 0, 0, 0);
+                }
+            };
+            // A NaN that some row does not see is taken out here and put into the rows that see it at the end; likewise values whose scale is not finite.
+            auto take_out = [&](uint4 (&c)[PASSES], const float* scales) {
+#pragma unroll 1
+                for (int p = 0; p < PASSES; ++p) {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int x = 0; x < PASSES; ++x)
+                        if (x == p) w = c[x];
+                    const bool finite = key_of(p) >= KEYS || fabsf(scales[min(key_of(p), KEYS - 1)]) < INFINITY;
+                    if (finite && !has_nan(w)) continue;
+                    sh.nan_values = 1;
+                    const uint32_t all = finite ? 0xffffffffu : 0u;
+                    w.x &= ~__vcmpeq4(w.x & 0x7f7f7f7fu, 0x7f7f7f7fu) & all;
+                    w.y &= ~__vcmpeq4(w.y & 0x7f7f7f7fu, 0x7f7f7f7fu) & all;
+                    w.z &= ~__vcmpeq4(w.z & 0x7f7f7f7fu, 0x7f7f7f7fu) & all;
+                    w.w &= ~__vcmpeq4(w.w & 0x7f7f7f7fu, 0x7f7f7f7fu) & all;
+#pragma unroll
+                    for (int x = 0; x < PASSES; ++x)
+                        if (x == p) c[x] = w;
+                }
+            };
+            // The codes of a block as fp16 numbers, times the ratio of their scale to the block's largest, into a stage.
+            auto put = [&](const uint4 (&c)[PASSES], unsigned char* stage, const float* scales, float inverse, bool careful) {
+#pragma unroll
+                for (int p = 0; p < PASSES; ++p) {
+                    const int key = key_of(p), col = col_of(p);
+                    if (key >= KEYS) continue;
+                    float ratio = scales[key] * inverse;
+                    if (careful && !(fabsf(ratio) < INFINITY)) ratio = 0.f;
+                    const __half2 r = __float2half2_rn(ratio);
+                    unsigned char* dst = stage + (col >> 2) * PANEL_BYTES + key * 128;
+                    // threads of the second panel begin with the second of their two 16-byte words: the eight of a key then write to different banks
+                    const int second = (col >> 2) & 1;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int word = (col & 3) * 2 + (i ^ second);
+                        const uint32_t x = i ^ second ? c[p].z : c[p].x, z = i ^ second ? c[p].w : c[p].y;
+                        uint32_t h[4] = {codes_to_f16(x), codes_to_f16_high(x), codes_to_f16(z), codes_to_f16_high(z)};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(h + j), r);
+                            h[j] = *reinterpret_cast<const uint32_t*>(&v);
+                        }
+                        *reinterpret_cast<uint4*>(dst + ((word ^ (key & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+            };
+            int page1 = page_for(1);
+            {
+                const int page0 = page_for(0);
+                put_info(0, page0, scale_of(a.k_scale, page0), scale_of(a.v_scale, page0));
+                put_info(1, page1, scale_of(a.k_scale, page1), scale_of(a.v_scale, page1));
+            }
+            int page2 = page_for(2);
+            loaders_meet();
+            ask(kc, a.k_cache, 0);
+            ask(vc, a.v_cache, 0);
+            bool ok = true;        // (a thread that has given up keeps meeting the others)
+            for (int b = 0; b < count; ++b) {
+                BlockInfo& f = sh.info[b % INFO];
+                const int st = b % STAGES;
+                const float ks = scale_of(a.k_scale, page2), vs = scale_of(a.v_scale, page2);      // of block b + 2
+                const int page3 = page_for(b + 3);
+                const float km = fmaxf(fmaxf(f.k_most[0], f.k_most[1]), fmaxf(f.k_most[2], f.k_most[3]));
+                const float vm = fmaxf(fmaxf(f.v_most[0], f.v_most[1]), fmaxf(f.v_most[2], f.v_most[3]));
+                if (lt == 0) {
+                    f.factor = km > 0.f ? km : 1.f;
+                    f.shift = vm > 0.f ? log2f(vm) - (float)base_exp : 0.f;
+                }
+                ok = ok && mbar_wait(sh.k_empty + st, ((b / STAGES) & 1) ^ 1);
+                put(kc, k_ring + st * TENSOR_BYTES, f.k_scale, km > 0.f ? 1.f / km : 1.f, false);
+                if (lane == 0) mbar_arrive(sh.k_full + st);
+                ask(kc, a.k_cache, b + 1);
+                ok = ok && mbar_wait(sh.v_empty + st, ((b / STAGES) & 1) ^ 1);
+                if (partial(b)) take_out(vc, f.v_scale);
+                put(vc, v_ring + st * TENSOR_BYTES, f.v_scale, vm > 0.f ? 1.f / vm : 1.f, partial(b));
+                if (lane == 0) mbar_arrive(sh.v_full + st);
+                ask(vc, a.v_cache, b + 1);
+                put_info(b + 2, page2, ks, vs);
+                page2 = page3;
+                loaders_meet();
+            }
+            if (!ok && lane == 0) oxr_report(a.status, OXR_WAIT_EXPIRED, 41);
+        } else if (one_lane()) {
+            // ------------------------------------------------------------------ the products
+            constexpr uint32_t idesc_s = idesc_of(HALF_ROWS, KEYS, false), idesc_o = idesc_of(HALF_ROWS, O_COLS, true);
+            const int halves = half1_live ? 2 : 1;
+            bool ok = count > 0;
+            auto wait_for = [&](uint64_t* bar, uint32_t parity, int where) -> bool {
+                if (!mbar_wait(bar, parity)) { oxr_report(a.status, OXR_WAIT_EXPIRED, where); return false; }
+                fence_after();
+                return true;
+            };
+            auto issue_s = [&](int b, int h) {
+                const uint32_t ka = smem_addr(k_ring + (b % STAGES) * TENSOR_BYTES), qa = smem_addr(q_tiles + h * TENSOR_BYTES);
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                    mma_smem(tmem + (uint32_t)(h * KEYS), desc_kmajor(qa + (kk >> 2) * PANEL_BYTES + (kk & 3) * 32), desc_kmajor(ka + (kk >> 2) * PANEL_BYTES + (kk & 3) * 32),
+                             idesc_s, kk > 0 ? 1u : 0u);
+                commit(sh.s_full + h);
+                if (h == halves - 1) commit(sh.k_empty + b % STAGES);
+            };
+            ok = ok && wait_for(&sh.q_ready, 0, 42) && wait_for(sh.k_full, 0, 43);
+            if (ok)
+                for (int h = 0; h < halves; ++h) issue_s(0, h);
+            // block by block and half by half: O_h += P_h(b) V(b), and at once S_h(b + 1) over the columns that P_h(b) was in (the pipe keeps their order)
+            for (int b = 0; b < count && ok; ++b) {
+                const uint32_t va = smem_addr(v_ring + (b % STAGES) * TENSOR_BYTES);
+                for (int h = 0; h < halves && ok; ++h) {
+                    ok = wait_for(sh.p_full + h, b & 1, 44) && (h > 0 || wait_for(sh.v_full + b % STAGES, (b / STAGES) & 1, 45));
+                    if (!ok) break;
+#pragma unroll
+                    for (int kk = 0; kk < KEYS / 16; ++kk)
+                        mma_tmem(tmem + 256 + (uint32_t)(h * O_COLS), tmem + (uint32_t)(h * KEYS + kk * 8), desc_mnmajor(va + kk * 16 * 128), idesc_o, (b > 0 || kk > 0) ? 1u : 0u);
+                    commit(sh.o_done + h);
+                    if (h == halves - 1) commit(sh.v_empty + b % STAGES);
+                    if (b + 1 < count) {
+                        ok = h > 0 || wait_for(sh.k_full + (b + 1) % STAGES, ((b + 1) / STAGES) & 1, 43);
+                        if (ok) issue_s(b + 1, h);
+                    }
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+        // ---------------------------------------------------------------------- softmax: a thread per row
+        const int half = (warp - 4) >> 2, quarter = warp & 3, rr = quarter * 32 + lane, r = half * HALF_ROWS + rr;
+        const int tok = r / a.heads_per_tile, head = hg * a.heads_per_tile + r % a.heads_per_tile;
+        const bool row_ok = r < rows && head < G;
+        const int row_pos = first_pos + tok, row_lo = a.window > 0 ? row_pos - a.window + 1 : 0;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const uint32_t tmem_s = tmem + lanes + (uint32_t)(half * KEYS), tmem_o = tmem + lanes + 256 + (uint32_t)(half * O_COLS);
+        float row_factor;
+        {   // the row as fp16 numbers, times the power of two that brings its largest entry to [2^14, 2^15)
+            const uint4* src = reinterpret_cast<const uint4*>(q + (size_t)(t.q_begin + t.tok0 + (row_ok ? tok : 0)) * a.q_stride + (size_t)(kvh * G + (row_ok ? head : 0)) * D);
+            uint4 v[D / 8];
+            float most = 0.f;
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+                v[c] = row_ok ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+                const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+            }
+            const int up = (most > 0.f && most < INFINITY) ? min(14 - (int)((__float_as_uint(most) >> 23) & 255) + 127, 126) : 0;
+            const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+            row_factor = a.scale * LOG2E * __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+                const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+                uint32_t h[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const __half2 x = __floats2half2_rn(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xffff0000u) * f);
+                    h[i] = *reinterpret_cast<const uint32_t*>(&x);
+                }
+                *reinterpret_cast<uint4*>(q_tiles + half * TENSOR_BYTES + (c >> 3) * PANEL_BYTES + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.q_ready);
+        }
+        if (half == 0 || half1_live) {
+            float m_used = -INFINITY, l = 0.f;      // of score + shift, in log2 units; the sum of 2^7 weights
+            bool alive = true;
+            for (int b = 0; b < count; ++b) {
+                if (!mbar_wait(sh.s_full + half, b & 1)) { if (lane == 0) oxr_report(a.status, OXR_WAIT_EXPIRED, 46); alive = false; break; }
+                fence_after();
+                const int key0 = (block0 + b) * KEYS;
+                // (never zero: a hidden score of -inf has to stay one)
+                const float factor = fmaxf(row_factor * sh.info[b % INFO].factor, 1e-37f), shift = sh.info[b % INFO].shift;
+                uint32_t sv[KEYS / 32][32];
+#pragma unroll
+                for (int c = 0; c < KEYS / 32; ++c) ld32(tmem_s + (uint32_t)(c * 32), sv[c]);
+                wait_ld();
+                // Rows without a token or head see what comes (their queries are zero); the others see keys row_lo .. row_pos.
+                if (key0 < row_lo || key0 + KEYS - 1 > row_pos) {
+                    const int from = row_lo - key0;
+                    const unsigned span = row_pos >= row_lo ? (unsigned)(row_pos - row_lo) : 0u;
+#pragma unroll
+                    for (int c = 0; c < KEYS / 32; ++c)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if ((unsigned)(c * 32 + j - from) > span || row_pos < row_lo) sv[c][j] = __float_as_uint(-INFINITY);
+                }
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < KEYS / 32; ++c)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) mx4[j & 3] = max3(mx4[j & 3], __uint_as_float(sv[c][2 * j]), __uint_as_float(sv[c][2 * j + 1]));
+                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * factor + shift;
+                float alpha = 1.f;
+                const bool raise = mx > m_used + RAISE || (m_used == -INFINITY && mx != -INFINITY);
+                if (raise) {
+                    alpha = m_used == -INFINITY ? 0.f : exp2_of(m_used - mx);
+                    m_used = mx;
+                }
+                // S(b) complete means that O += P(b - 1) V(b - 1), issued before it, is complete: O may be rescaled
+                if (__any_sync(0xffffffffu, raise && b > 0)) {
+#pragma unroll 1
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t ov[16];
+                        ld16(tmem_o + (uint32_t)(c * 16), ov);
+                        wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * alpha);
+                        st16(tmem_o + (uint32_t)(c * 16), ov);
+                    }
+                    wait_st();
+                }
+                const float off = (m_used == -INFINITY ? 0.f : shift - m_used) + P_SHIFT;
+                const uint64_t factor2 = pair_of(factor, factor), off2 = pair_of(off, off);
+                uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+                for (int c = 0; c < KEYS / 32; ++c) {
+                    uint32_t pv[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        float x0, x1;
+                        unpair(fma2(pair_of(__uint_as_float(sv[c][2 * e]), __uint_as_float(sv[c][2 * e + 1])), factor2, off2), x0, x1);
+                        const float p0 = exp2_of(x0), p1 = exp2_of(x1);
+                        sum2[e & 3] = add2(sum2[e & 3], pair_of(p0, p1));
+                        const __half2 pk = __floats2half2_rn(p0, p1);
+                        pv[e] = *reinterpret_cast<const uint32_t*>(&pk);
+                    }
+                    st16(tmem_s + (uint32_t)(c * 16), pv);
+                }
+                float sum4[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { float x, z; unpair(sum2[i], x, z); sum4[i] = x + z; }
+                wait_st();
+                l = l * alpha + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3])) * exp2_of(-shift);
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sh.p_full + half);
+            }
+            // ---- O / l
+            if (alive && count > 0 && !mbar_wait(sh.o_done + half, (count - 1) & 1)) { if (lane == 0) oxr_report(a.status, OXR_WAIT_EXPIRED, 47); alive = false; }
+            alive = __all_sync(0xffffffffu, alive);
+            if (alive) {
+                fence_after();
+                const float inverse = 1.f / l, unscale = exp2_of((float)base_exp);
+                __nv_bfloat16* dst = out + ((size_t)(t.q_begin + t.tok0 + tok) * a.H + (size_t)kvh * G + head) * D;
+#pragma unroll 1
+                for (int c = 0; c < D / 16; ++c) {
+                    uint32_t ov[16];
+                    if (count > 0) {
+                        ld16(tmem_o + (uint32_t)(c * 16), ov);
+                        wait_ld();
+                    }
+                    uint4 o4[2];
+                    __nv_bfloat162* op = reinterpret_cast<__nv_bfloat162*>(o4);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        op[e] = l == 0.f ? __floats2bfloat162_rn(0.f, 0.f)
+                                         : __floats2bfloat162_rn(__uint_as_float(ov[2 * e]) * inverse * unscale, __uint_as_float(ov[2 * e + 1]) * inverse * unscale);
+                    if (row_ok) {
+                        reinterpret_cast<uint4*>(dst + 16 * c)[0] = o4[0];
+                        reinterpret_cast<uint4*>(dst + 16 * c)[1] = o4[1];
+                    }
+                }
+                // values that were taken out of blocks which not every row sees: NaN to the rows that do
+                if (*reinterpret_cast<volatile int*>(&sh.nan_values) && row_ok) {
+                    for (int key = max(row_lo, block0 * KEYS); key <= min(row_pos, hi - 1); ++key) {
+                        if (!partial(key / KEYS - block0)) { key = key / KEYS * KEYS + KEYS - 1; continue; }
+                        const int page = __ldg(table_row + a.page_of(key));
+                        if (page < 0 || page >= a.num_pages) continue;
+                        const bool finite = fabsf(__ldg(a.v_scale + (size_t)page * a.KV + kvh)) < INFINITY;
+                        const unsigned char* codes = a.v_cache + (long long)page * a.page_stride + (a.in_page(key) * a.KV + kvh) * D;
+                        for (int d = 0; d < D; ++d)
+                            if (!finite || (__ldg(codes + d) & 0x7f) == 0x7f) dst[d] = __float2bfloat16_rn(__uint_as_float(0x7fffffffu));
+                    }
+                }
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
+}
+}  // namespace
+#endif
+
+// As oxr_kv8_attention, for bf16 queries, head sizes up to 128 and a positive scale; `tiles`: at least as many as the requests make of 256 rows.
+OXR_API int oxr_kv8_prompt_attention(void* out, const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, const int* cu_q,
+                                     const int* ctx_lens, const int* block_table, int n, int n_tokens, int table_width, int page_size, long long page_stride,
+                                     int num_pages, int H, int KV, long long q_stride, float scale, int window, int min_q, int max_q, int any_q, int tiles,
+                                     int* status, cudaStream_t stream) {
+#if HEAD_DIM <= 128
+    if (n < 0 || n_tokens < 0 || KV <= 0 || H <= 0 || H % KV || page_size <= 0 || table_width < 0 || num_pages < 0 || window < 0 || tiles < 0) return OXR_BAD_ARGUMENT;
+    if (any_q < 2 || min_q < 1 || !(scale > 0.f)) return OXR_BAD_ARGUMENT;
+    if (tiles == 0 || n == 0 || n_tokens == 0) return 0;
+    const Kv8Args a = kv8_args(k_cache, v_cache, k_scale, v_scale, cu_q, ctx_lens, block_table, n, n_tokens, table_width, page_size, page_stride, num_pages, H,
+                               KV, q_stride, scale, window, min_q, max_q, any_q, TILE_ROWS, status);
+    const long long grid = (long long)tiles * KV * a.head_groups;
+    if (grid > 0x7fffffffll) return OXR_BAD_ARGUMENT;
+    static thread_local int ready = -1;
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return oxr_launch_status();
+    if (ready != device) {
+        // setmaxnreg deals out what the block is launched with: 128 registers a thread, or the softmax warps would wait for theirs in vain
+        cudaFuncAttributes attrs;
+        if (cudaFuncGetAttributes(&attrs, attn_kv8_prompt_kernel) != cudaSuccess) return oxr_launch_status();
+        if (attrs.numRegs != 128) return OXR_BAD_ARGUMENT;
+        if (cudaFuncSetAttribute(attn_kv8_prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM) != cudaSuccess) return oxr_launch_status();
+        ready = device;
+    }
+    oxr_launch(attn_kv8_prompt_kernel, dim3((unsigned)grid), dim3(THREADS), SMEM, stream, true, (__nv_bfloat16*)out, (const __nv_bfloat16*)q, a, tiles);
+    return oxr_launch_status();
+#else
+    return OXR_BAD_ARGUMENT;
+#endif
+}

@@ -31,7 +31,7 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompil
 CORE_SOURCES = ["elementwise.cu", "qk_norm_rope.cu", "gemm_f32.cu", "gemm_f32_short.cu", "gemm_skinny.cu", "gemm_stream.cu", "gemm_tcgen05.cu", "gemm_tcgen05_pair.cu", "gemm_tcgen05_few_rows.cu", "sampling.cu",
                 "stream_ops.cu", "mamba.cu", "attention_rows.cu", "attention_mix.cu", "attention_mix_mma.cu", "conv_qkv.cu", "mlstm.cu", "experts.cu", "head_prep.cu", "gla.cu", "shift_norm.cu", "delta.cu", "differential.cu", "hyper.cu", "kv8.cu"]
 ATTENTION_SOURCES = ["attention.cu"]
-KV8_SOURCES = ["attention_kv8.cu"]
+KV8_SOURCES = ["attention_kv8.cu", "attention_kv8_prompt.cu"]
 HEADERS = ["attention_kv8.cuh", "common.cuh", "scan_columns.cuh", "tma.cuh", "umma.cuh", "sampling_static.h"]
 
 

@@ -32,6 +32,8 @@ def _kv8_lib(head_dim: int):
         p, i, f, ll = c_void_p, c_int, c_float, c_longlong
         lib.oxr_kv8_attention.argtypes = [p] * 9 + [i, i, i, i, ll, i, i, i, ll, f, i, i, i, i, i, i, p, i, p, p]
         lib.oxr_kv8_attention.restype = c_int
+        lib.oxr_kv8_prompt_attention.argtypes = [p] * 9 + [i, i, i, i, ll, i, i, i, ll, f, i, i, i, i, i, p, p]
+        lib.oxr_kv8_prompt_attention.restype = c_int
         lib.oxr_kv8_blocks_per_sm.argtypes = [i, i]
         lib.oxr_kv8_blocks_per_sm.restype = c_int
         lib.oxr_kv8_head_dim.restype = c_int
@@ -141,6 +143,26 @@ def kv8_blocks(tiles: int, key_blocks: int, room: int) -> int:
     return max(1, min(room, -(-tiles * key_blocks // 4)))
 
 
+KV8_PROMPT_ROWS = 256
+"""Rows of a tile of the tcgen05 kernel for long portions."""
+KV8_PROMPT_TILES = 24
+"""From how many such tiles on that kernel takes a step's portions of more than ``ops.SHORT_MAX_TOKENS`` tokens. A tile walks over its keys alone, so a few of them
+leave most of the GPU idle. Measured on a B200 (32 / 8 heads of 128), that kernel against the split-key one: 8 tiles on 4,096 keys 87 and 49 us, 16 on 8,192 keys 160
+and 125, 32 on 4,096 keys 88 and 129, 64 on 512 keys 24 and 52."""
+
+
+def kv8_prompt_tiles(tokens: int, max_q_len: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, scale: float) -> int:
+    """Tiles that the tcgen05 kernel would have to do for one KV head's query heads, about; 0 where the split-key kernel does the whole step: other types and
+    sizes, a scale that is not positive (the row's maximum is scaled, not each score), short portions, or too few tiles."""
+    if dtype != torch.bfloat16 or head_dim > 128 or not scale > 0 or max_q_len <= ops.SHORT_MAX_TOKENS:
+        return 0
+    group = num_heads // num_kv_heads
+    heads_per_tile = min(group, KV8_PROMPT_ROWS)
+    per_tile = KV8_PROMPT_ROWS // heads_per_tile
+    tiles = max(-(-max_q_len // per_tile), tokens // per_tile)
+    return tiles if tiles * num_kv_heads * -(-group // heads_per_tile) >= KV8_PROMPT_TILES else 0
+
+
 def paged_attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, *,
                         cu_q: torch.Tensor, ctx_lens: torch.Tensor, block_table: torch.Tensor, scale: float, window: int = 0, max_q_len: int,
                         kv_len_bound: int, status: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -174,17 +196,24 @@ def paged_attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         return out
     lib = _kv8_lib(d)
     group = heads // kv
-    rows = 8 if group * max_q_len <= 8 else 16      # the split-key kernel's tiles: (token, query head) pairs of one KV head
+    common = (out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), cu_q.data_ptr(), ctx_lens.data_ptr(),
+              block_table.data_ptr(), n, tokens, block_table.shape[1], page, page_stride, pages, heads, kv, q_stride, float(scale), int(window))
+    longest = max_q_len = int(max_q_len)
+    if kv8_prompt_tiles(tokens, max_q_len, heads, kv, d, q.dtype, scale):
+        fewest = ops.SHORT_MAX_TOKENS + 1 if n > 1 else 1      # a request alone goes there whatever it brings
+        tiles = min(tokens, min(n, tokens // fewest) + tokens // (KV8_PROMPT_ROWS // min(group, KV8_PROMPT_ROWS)))
+        ops._done(lib.oxr_kv8_prompt_attention(*common, fewest, max_q_len, max_q_len, tiles, status.data_ptr(), ops._stream()), "paged_attention_kv8 (prompts)")
+        longest = fewest - 1
+        if longest == 0:
+            return out
+    rows = 8 if group * longest <= 8 else 16      # the split-key kernel's tiles: (token, query head) pairs of one KV head
     heads_per_tile = min(group, rows)
     per_tile = rows // heads_per_tile
-    tiles = min(tokens, n * -(-max_q_len // per_tile), n + tokens // per_tile) * kv * -(-group // heads_per_tile)
-    seen = min(kv_len_bound, window + max_q_len + 32) if window > 0 else kv_len_bound
+    tiles = min(tokens, n * -(-longest // per_tile), n + tokens // per_tile) * kv * -(-group // heads_per_tile)
+    seen = min(kv_len_bound, window + longest + 32) if window > 0 else kv_len_bound
     blocks = kv8_blocks(tiles, max(1, -(-seen // 32)), _kv8_room(d, code, rows))
     scratch = torch.empty(8 * blocks * rows * (d + 2) + 32 * blocks, dtype=torch.float32, device=q.device)
-    ops._done(lib.oxr_kv8_attention(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                                    cu_q.data_ptr(), ctx_lens.data_ptr(), block_table.data_ptr(), n, tokens, block_table.shape[1], page, page_stride, pages,
-                                    heads, kv, q_stride, float(scale), int(window), 1, int(max_q_len), int(max_q_len), rows, blocks, scratch.data_ptr(), code,
-                                    status.data_ptr(), ops._stream()), "paged_attention_kv8")
+    ops._done(lib.oxr_kv8_attention(*common, 1, longest, max_q_len, rows, blocks, scratch.data_ptr(), code, status.data_ptr(), ops._stream()), "paged_attention_kv8")
     ops.launch_count += 1
     return out
 

@@ -82,11 +82,12 @@ def attention(q, k_codes, v_codes, k_scale, v_scale, q_lens, ctx_lens, tables, s
 
 
 def tolerance(out, spread, size, dtype, head_dim, keys):
-    """How far a kernel may be off. The result is rounded to its type; weights are rounded to 11 (bf16) or 22 bits (fp32) and come from an exp2 good to
+    """How far a kernel may be off. The result is rounded to its type; weights are rounded to one fp16 number (bf16 queries) or two of
+    them (fp32): an fp16 number has 11 significant bits, half a step is 2^-11 of a number just above a power of two, and the second number leaves 2^-11 of that; they come from an exp2 good to
     2^-22 twice (numerator and denominator); a score's fp32 sum of ``head_dim`` products and its two factors err by 2^-22 of the sum of their
     magnitudes each at most (the tensor cores cut instead of rounding), which moves a weight by as much; and the sum over the keys, 16 at a time, errs in the same way."""
     half = torch.finfo(dtype).eps / 2
-    weight = 2.0 ** (-12 if dtype == torch.bfloat16 else -23) + 2 * 2.0 ** -22 + 2 * (head_dim / 16 + 8) * 2.0 ** -22 * size + (keys / 16 + 20) * 2.0 ** -22
+    weight = 2.0 ** (-11 if dtype == torch.bfloat16 else -22) + 2 * 2.0 ** -22 + 2 * (head_dim / 16 + 8) * 2.0 ** -22 * size + (keys / 16 + 20) * 2.0 ** -22
     return half * out.abs() + weight * spread * 1.01 + 1e-37
 
 
