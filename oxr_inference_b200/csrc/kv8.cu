@@ -12,20 +12,11 @@ namespace {
 // fall below e4m3's normal range. Powers of two cost e4m3 nothing (its precision does not depend on where in its range a number lies) and make
 // the result independent of how a request's tokens were cut into calls, but for those entries.
 //
-// One block works on a page: the block of the first token in the call that names it. (A token whose predecessor names the same page is not the
-// first; the others look through all slots before their own, then gather the page's tokens from those behind.) So any order of slots is taken, nothing
-// is shared between blocks, and of two tokens with one slot the later one stays. What bounds it: reading x and writing the codes; in a decode step
-// the launch.
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(u[i] << 16); v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
-}
+// One block works on a page (of two KV heads): that of the first token in the call that names it. (A token whose predecessor names the same page is not
+// the first; for the others the block looks through all slots before, then gathers the page's tokens from those behind, or, where the tokens are
+// many, another kernel has found the first and the last token of each page.) So any order of slots is taken, nothing is shared between blocks,
+// and of two tokens with one slot the later one stays. A warp has one head's keys or values of the page: their
+// largest magnitude, then the codes, from registers where they fit. What bounds it: reading x and writing the codes; in a decode step the launch.
 __device__ __forceinline__ uint2 codes_of(const float (&v)[8]) {
     uint32_t h[4];
 #pragma unroll
@@ -57,83 +48,204 @@ struct Kv8Pool {
     long long x_stride;     // entries from token to token
 };
 
-template <typename T>
-__global__ void store_kv8_kernel(const Kv8Pool kp, const Kv8Pool vp, const int* __restrict__ slots, int n, long long page_stride, int num_pages, int page_size,
-                                 int KV, int D, int heads_per_block, int* status) {
+// Eight entries as they come.
+template <typename T> struct Raw;
+template <> struct Raw<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) { a = __ldg(reinterpret_cast<const float4*>(p)); b = __ldg(reinterpret_cast<const float4*>(p) + 1); }
+    __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+    // the largest of `bits` and the magnitudes, compared as integers (infinities and NaN then lie above all numbers)
+    __device__ __forceinline__ uint32_t most(uint32_t bits) const {
+        float v[8];
+        get(v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) bits = max(bits, __float_as_uint(v[i]) & 0x7fffffffu);
+        return bits;
+    }
+    static __device__ __forceinline__ uint32_t as_float(uint32_t bits) { return bits; }
+    __device__ __forceinline__ void get(float (&v)[8]) const { v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w; }
+};
+template <> struct Raw<__nv_bfloat16> {
+    uint4 w;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { w = __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ uint32_t most(uint32_t bits) const {      // two 16-bit numbers
+        constexpr uint32_t M = 0x7fff7fffu;
+        return __vmaxu2(__vmaxu2(__vmaxu2(bits, w.x & M), __vmaxu2(w.y & M, w.z & M)), w.w & M);
+    }
+    static __device__ __forceinline__ uint32_t as_float(uint32_t bits) { return max(bits << 16, bits & 0xffff0000u); }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(u[i] << 16); v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+    }
+};
+
+// Which tokens of the call name a page, for calls of many tokens: the first and the last of them. `ends` [num_pages][2] comes as -1.
+__global__ void store_kv8_ends_kernel(int* __restrict__ ends, const int* __restrict__ slots, int n, int page_size, int num_pages) {
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    const int s = i < n ? __ldg(slots + i) : -1;
+    if (s < 0 || s / page_size >= num_pages) return;
+    const int page = s / page_size, before = i > 0 ? __ldg(slots + i - 1) : -1, after = i + 1 < n ? __ldg(slots + i + 1) : -1;
+    if (before < 0 || before / page_size != page) atomicMin(reinterpret_cast<unsigned*>(ends) + 2 * page, (unsigned)i);
+    if (after < 0 || after / page_size != page) atomicMax(ends + 2 * page + 1, i);
+}
+
+constexpr int FEW_TOKENS = 1024;
+constexpr int HELD = 8;   // groups of eight entries that a lane keeps between the two looks at them: pages of up to 2,048 entries a head
+
+// EIGHTS: D / 8 where that divides a warp, else 0 (taken from D).
+template <typename T, int EIGHTS>
+__global__ void __launch_bounds__(128, sizeof(T) == 4 ? 4 : 6) store_kv8_kernel(const Kv8Pool kp, const Kv8Pool vp, const int* __restrict__ slots, const int* __restrict__ ends, int n,
+                                                           long long page_stride, int num_pages, int page_size, int KV, int D, int tokens_per_block, int* status) {
     extern __shared__ int winner[];   // [page_size] the token that is stored at each place of the page, or -1
     pdl_wait();
     pdl_trigger();
-    const int i = blockIdx.x;
-    const int slot = __ldg(slots + i);
-    if (slot < 0) return;
-    const int page = slot / page_size;
-    if (page >= num_pages) {
-        if (threadIdx.x == 0 && blockIdx.y == 0) oxr_report(status, OXR_BAD_SLOT, i);
-        return;
-    }
-    const int first = page * page_size;   // below 2^31: `slot` is
-    auto here = [&](int s) { return (unsigned)(s - first) < (unsigned)page_size; };   // (negative slots wrap far above)
-    if (i > 0 && here(__ldg(slots + i - 1))) return;
-    bool earlier = false;
-#pragma unroll 8
-    for (int j = threadIdx.x; j < i - 1; j += blockDim.x) earlier |= here(__ldg(slots + j));
-    for (int j = threadIdx.x; j < page_size; j += blockDim.x) winner[j] = -1;
-    if (__syncthreads_or(earlier)) return;
-#pragma unroll 8
-    for (int j = i + threadIdx.x; j < n; j += blockDim.x) {
-        const int s = __ldg(slots + j);
-        if (here(s)) atomicMax(winner + (s - first), j);
-    }
-    __syncthreads();
-    const bool begun = winner[0] >= 0;
-
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int eights = D / 8, items = page_size * eights;
-    const int h0 = blockIdx.y * heads_per_block, h1 = min(KV, h0 + heads_per_block);
-    for (int u = 2 * h0 + warp; u < 2 * h1; u += warps) {
-        const int h = u >> 1;
-        const Kv8Pool& pool = (u & 1) ? vp : kp;
-        const T* x = reinterpret_cast<const T*>(pool.x) + (size_t)h * D;
-        unsigned char* cache = pool.cache + (long long)page * page_stride + (size_t)h * D;
-        float most = 0.f;
-#pragma unroll 4
-        for (int e = lane; e < items; e += 32) {
-            const int t = winner[e / eights];
-            if (t < 0) continue;
-            float v[8];
-            load8(x + t * pool.x_stride + e % eights * 8, v);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float f = fabsf(v[k]);
-                if (f < INFINITY) most = fmaxf(most, f);   // neither infinities nor NaN have a say
-            }
-        }
-        most = warp_max(most);
-        float* where = pool.scale + (size_t)page * KV + h;
-        const float old = begun ? 0.f : *where;
-        const float scale = fmaxf(old, scale_for(most));
-        const bool again = !begun && scale > old;
-        const float ratio = again ? old / scale : 1.f, inverse = scale > 0.f ? 1.f / scale : 0.f;
-#pragma unroll 4
-        for (int e = lane; e < items; e += 32) {
-            const int off = e / eights, t = winner[off];
-            uint2* at = reinterpret_cast<uint2*>(cache + (size_t)off * KV * D + e % eights * 8);
-            float v[8];
-            if (t >= 0) {
-                load8(x + t * pool.x_stride + e % eights * 8, v);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = fabsf(v[k]) < INFINITY ? v[k] * inverse : __uint_as_float(0x7fffffffu);   // e4m3 has no infinity
-            } else if (again) {
-                values_of(*at, v);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] *= ratio;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int eights = EIGHTS ? EIGHTS : D / 8;
+    // which of the block's tokens (32 at most) begin a run of tokens of one page
+    const int i0 = blockIdx.x * tokens_per_block;
+    bool begins = false;
+    if (lane < tokens_per_block && i0 + lane < n) {
+        const int s = __ldg(slots + i0 + lane), before = i0 + lane > 0 ? __ldg(slots + i0 + lane - 1) : -1;
+        if (s >= 0) {
+            const int page = s / page_size;
+            if (page >= num_pages) {
+                if (warp == 0 && blockIdx.y == 0) oxr_report(status, OXR_BAD_SLOT, i0 + lane);
             } else {
-                continue;
+                begins = (before < 0 || before / page_size != page) && (ends == nullptr || __ldg(ends + 2 * page) == i0 + lane);
             }
-            *at = codes_of(v);
         }
-        __syncwarp();
-        if (lane == 0) *where = scale;
+    }
+    for (unsigned runs = __ballot_sync(0xffffffffu, begins); runs; runs &= runs - 1) {     // the same in every warp
+        const int i = i0 + __ffs(runs) - 1;
+        const int page = __ldg(slots + i) / page_size, first = page * page_size;   // below 2^31, as the slot is
+        auto here = [&](int s) { return (unsigned)(s - first) < (unsigned)page_size; };   // (negative slots wrap far above)
+        const int u = 2 * blockIdx.y * 2 + warp, h = u >> 1;      // this warp's head and whether it has the keys or the values
+        const Kv8Pool& pool = (u & 1) ? vp : kp;
+        const unsigned x_stride = (unsigned)pool.x_stride;
+        float* where = pool.scale + (size_t)page * KV + h;
+        const float before = h < KV ? *where : 0.f;
+        const int last = ends != nullptr ? __ldg(ends + 2 * page + 1) : n - 1;
+        for (int j = threadIdx.x; j < page_size; j += blockDim.x) winner[j] = -1;
+        if (ends == nullptr) {
+            bool earlier = false;
+#pragma unroll 8
+            for (int j = threadIdx.x; j < i - 1; j += blockDim.x) earlier |= here(__ldg(slots + j));
+            if (__syncthreads_or(earlier)) continue;      // the page is another block's
+        } else {
+            __syncthreads();
+        }
+#pragma unroll 8
+        for (int j = i + threadIdx.x; j <= last; j += blockDim.x) {
+            const int s = __ldg(slots + j);
+            if (here(s)) atomicMax(winner + (s - first), j);
+        }
+        __syncthreads();
+        const bool begun = winner[0] >= 0;
+        const int items = page_size * eights;
+        if (h < KV) {
+            const T* x = reinterpret_cast<const T*>(pool.x) + (size_t)h * D;
+            unsigned char* cache = pool.cache + (long long)page * page_stride + (size_t)h * D;
+            const float old = begun ? 0.f : before;
+            const bool hold = items <= 32 * HELD;
+            auto from = [&](int e, int t) { return x + (size_t)(unsigned)t * x_stride + e % eights * 8; };
+            auto to = [&](int e) { return reinterpret_cast<uint2*>(cache + (unsigned)(e / eights * KV * D + e % eights * 8)); };
+            Raw<T> held[HELD];
+            int token[HELD];
+            uint32_t bits = 0u;
+            if (hold) {
+#pragma unroll
+                for (int c = 0; c < HELD; ++c) token[c] = c * 32 + lane < items ? winner[(c * 32 + lane) / eights] : -1;
+#pragma unroll
+                for (int c = 0; c < HELD; ++c) {
+                    held[c].zero();
+                    if (token[c] >= 0) held[c].load(from(c * 32 + lane, token[c]));
+                }
+#pragma unroll
+                for (int c = 0; c < HELD; ++c) bits = held[c].most(bits);
+            } else {
+#pragma unroll 4
+                for (int e = lane; e < items; e += 32) {
+                    const int t = winner[e / eights];
+                    if (t < 0) continue;
+                    Raw<T> r;
+                    r.load(from(e, t));
+                    bits = r.most(bits);
+                }
+            }
+            bits = __reduce_max_sync(0xffffffffu, Raw<T>::as_float(bits));
+            const bool odd = bits >= 0x7f800000u;      // infinities or NaN, which have no say
+            float most = __uint_as_float(bits);
+            if (odd) {
+                most = 0.f;
+                for (int e = lane; e < items; e += 32) {
+                    const int t = winner[e / eights];
+                    if (t < 0) continue;
+                    Raw<T> r;
+                    float w[8];
+                    r.load(from(e, t));
+                    r.get(w);
+                    for (int k = 0; k < 8; ++k)
+                        if (fabsf(w[k]) < INFINITY) most = fmaxf(most, fabsf(w[k]));
+                }
+                most = warp_max(most);
+            }
+            const float scale = fmaxf(old, scale_for(most));
+            const bool again = !begun && scale > old;
+            const float inverse = scale > 0.f ? 1.f / scale : 0.f;
+            if (hold && !odd) {
+#pragma unroll
+                for (int c = 0; c < HELD; ++c)
+                    if (token[c] >= 0) {
+                        float w[8];
+                        held[c].get(w);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) w[k] *= inverse;
+                        *to(c * 32 + lane) = codes_of(w);
+                    }
+            } else {
+                for (int e = lane; e < items; e += 32) {
+                    const int t = winner[e / eights];
+                    if (t < 0) continue;
+                    Raw<T> r;
+                    float w[8];
+                    r.load(from(e, t));
+                    r.get(w);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) w[k] = fabsf(w[k]) < INFINITY ? w[k] * inverse : __uint_as_float(0x7fffffffu);   // e4m3 has no infinity
+                    *to(e) = codes_of(w);
+                }
+            }
+            if (again) {       // what the page holds already, to the new scale
+                const float ratio = old / scale;
+                for (int e = lane; e < items; e += 32) {
+                    if (winner[e / eights] >= 0) continue;
+                    float w[8];
+                    values_of(*to(e), w);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) w[k] *= ratio;
+                    *to(e) = codes_of(w);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) *where = scale;
+        }
+        __syncthreads();      // `winner` is read
+    }
+}
+
+template <typename T>
+void launch_store(dim3 grid, size_t smem, cudaStream_t stream, const Kv8Pool& kp, const Kv8Pool& vp, const int* slots, const int* ends, int n, long long page_stride,
+                  int num_pages, int page_size, int KV, int D, int tokens, int* status) {
+    auto go = [&](auto kernel) { oxr_launch(kernel, grid, dim3(128), smem, stream, true, kp, vp, slots, ends, n, page_stride, num_pages, page_size, KV, D, tokens, status); };
+    switch (D) {
+        case 16: go(store_kv8_kernel<T, 2>); break;
+        case 32: go(store_kv8_kernel<T, 4>); break;
+        case 64: go(store_kv8_kernel<T, 8>); break;
+        case 128: go(store_kv8_kernel<T, 16>); break;
+        case 256: go(store_kv8_kernel<T, 32>); break;
+        default: go(store_kv8_kernel<T, 0>);
     }
 }
 
@@ -291,24 +403,31 @@ __global__ void __launch_bounds__(PAGE_THREADS) step_pages_kernel(const StepPage
 }
 }  // namespace
 
-// k, v [n, KV, D] (tokens k_stride / v_stride entries apart, rows 16-byte aligned) -> slots of the pools. dtype 0: fp32, 1: bf16.
+// k, v [n, KV, D] (tokens k_stride / v_stride entries apart, rows 16-byte aligned) -> slots of the pools. dtype 0: fp32, 1: bf16. `ends`: scratch of
+// [num_pages][2] words, needed for more than FEW_TOKENS tokens.
 OXR_API int oxr_store_kv8(void* k_cache, void* v_cache, float* k_scale, float* v_scale, const void* k, const void* v, long long k_stride, long long v_stride,
-                          const int* slots, int n, long long page_stride, int num_pages, int page_size, int KV, int D, int dtype, int* status, cudaStream_t stream) {
+                          const int* slots, int n, long long page_stride, int num_pages, int page_size, int KV, int D, int dtype, int* ends, int* status,
+                          cudaStream_t stream) {
     if (n < 0 || num_pages < 0 || page_size <= 0 || page_size > 8192 || KV <= 0 || D <= 0 || D % 16 || (dtype != 0 && dtype != 1)) return OXR_BAD_ARGUMENT;
+    if (k_stride < 0 || v_stride < 0 || k_stride > 0x7fffffffll || v_stride > 0x7fffffffll || (long long)page_size * KV * D > 0x7fffffffll) return OXR_BAD_ARGUMENT;
     if (n == 0) return 0;
     const Kv8Pool kp = {(unsigned char*)k_cache, k_scale, k, k_stride}, vp = {(unsigned char*)v_cache, v_scale, v, v_stride};
-    // Few tokens, most of them alone on their pages: a block per two KV heads (64 tokens of 8 heads of 128 are then 256 blocks). Many tokens fill the
-    // GPU with their pages alone, and one block saves the others the search for the page's tokens.
-    const bool few = n <= 1024;
-    const int heads = few ? (KV < 2 ? KV : 2) : KV, threads = few ? 128 : 256;
-    const dim3 grid(n, (KV + heads - 1) / heads);
+    // Few tokens, most of them alone on their pages: a block per token and two KV heads, which looks through all slots itself. Many tokens: a first
+    // kernel finds each page's first and last token, and a block looks after 16 tokens, a page or two.
+    const bool few = n <= FEW_TOKENS;
+    if (!few) {
+        if (ends == nullptr) return OXR_BAD_ARGUMENT;
+        if (cudaMemsetAsync(ends, 0xff, (size_t)num_pages * 2 * sizeof(int), stream) != cudaSuccess) return oxr_launch_status();
+        oxr_launch(store_kv8_ends_kernel, dim3((n + 255) / 256), dim3(256), 0, stream, false, ends, slots, n, page_size, num_pages);
+    }
+    const int tokens = few ? 1 : 16;
+    const dim3 grid((n + tokens - 1) / tokens, (KV + 1) / 2);
     const size_t smem = (size_t)page_size * sizeof(int);
-    if (dtype == 0)
-        oxr_launch(store_kv8_kernel<float>, grid, dim3(threads), smem, stream, true, kp, vp, slots, n, page_stride, num_pages, page_size, KV, D, heads, status);
-    else
-        oxr_launch(store_kv8_kernel<__nv_bfloat16>, grid, dim3(threads), smem, stream, true, kp, vp, slots, n, page_stride, num_pages, page_size, KV, D, heads, status);
+    if (dtype == 0) launch_store<float>(grid, smem, stream, kp, vp, slots, few ? nullptr : ends, n, page_stride, num_pages, page_size, KV, D, tokens, status);
+    else launch_store<__nv_bfloat16>(grid, smem, stream, kp, vp, slots, few ? nullptr : ends, n, page_stride, num_pages, page_size, KV, D, tokens, status);
     return oxr_launch_status();
 }
+OXR_API int oxr_store_kv8_few() { return FEW_TOKENS; }
 
 OXR_API int oxr_step_pages(int* lengths, int* held, int* table, int* free_list, int* free_count, const int* q_lens, const int* fresh, int rows, int width,
                            int page_size, int pool, int tokens, int* slots, int* positions, int* req_of_token, int* cu_q, int* ctx_lens, int advance, int* status,

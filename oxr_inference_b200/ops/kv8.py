@@ -19,7 +19,9 @@ from oxr_inference_b200.ops import build
 from oxr_inference_b200.ops.build import BuildError
 
 KV8_DTYPE = torch.float8_e4m3fn
-_INT = torch.int32
+KV8_FEW_TOKENS = 1024
+"""Up to so many tokens the store looks through all slots itself; for more it takes scratch of two words a page."""
+_INT, _F32 = torch.int32, torch.float32
 
 _kv8: dict = {}
 _core = None
@@ -51,10 +53,12 @@ def _core_lib():
     if _core is None:
         lib = ops._lib()
         p, i, ll = c_void_p, c_int, c_longlong
-        lib.oxr_store_kv8.argtypes = [p, p, p, p, p, p, ll, ll, p, i, ll, i, i, i, i, i, p, p]
+        lib.oxr_store_kv8.argtypes = [p, p, p, p, p, p, ll, ll, p, i, ll, i, i, i, i, i, p, p, p]
         lib.oxr_store_kv8.restype = c_int
         lib.oxr_step_pages.argtypes = [p] * 7 + [i] * 5 + [p] * 5 + [i, p, p]
         lib.oxr_step_pages.restype = c_int
+        if lib.oxr_store_kv8_few() != KV8_FEW_TOKENS:
+            raise BuildError(f"the store's kernels take up to {lib.oxr_store_kv8_few()} tokens without scratch, the host {KV8_FEW_TOKENS}")
         _core = lib
     return _core
 
@@ -67,26 +71,32 @@ def _here(t: torch.Tensor, name: str) -> None:
         raise ops.KernelError(f"{name} is on {t.device}, the current device is cuda:{ops._raw_device()}")
 
 
-def _need_all(device: int, dtype: torch.dtype, **tensors: torch.Tensor) -> None:
+# The checks are laid out for calls that pass them: a few comparisons in one expression each, and a function that finds the words for one that does not.
+# (Outside of CUDA graphs a small step's calls are bound by the host: this brought them from 19-23 to MEASURED.)
+def _plain(t: torch.Tensor, device: int, dtype: torch.dtype) -> bool:
+    return t.dtype is dtype and t.is_contiguous() and t.get_device() == device
+
+
+def _refuse_plain(device: int, dtype: torch.dtype, **tensors: torch.Tensor) -> None:
     for name, t in tensors.items():
-        if t.get_device() != device or t.dtype != dtype or not t.is_contiguous():
+        if not _plain(t, device, dtype):
             raise ops.KernelError(f"{name} must be contiguous {dtype} on cuda:{device}, got {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
 
 
 def _need_pools(device: int, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> tuple[int, int, int, int, int]:
     """(pages, page size, KV heads, head size, bytes from page to page) of the pools, which may be slices of wider ones as long as each page is whole."""
     shape, strides = k_cache.shape, k_cache.stride()
-    if len(shape) != 4 or k_cache.dtype != KV8_DTYPE or v_cache.dtype != KV8_DTYPE or v_cache.shape != shape:
+    if len(shape) != 4 or k_cache.dtype is not KV8_DTYPE or v_cache.dtype is not KV8_DTYPE or v_cache.shape != shape:
         raise ops.KernelError(f"the pools must be [pages, page size, KV heads, head size] of {KV8_DTYPE}, got {k_cache.dtype} {tuple(shape)} and "
                               f"{v_cache.dtype} {tuple(v_cache.shape)}")
     pages, page, kv, d = shape
-    whole = page * kv * d
-    if (strides[1:] != (kv * d, d, 1) or v_cache.stride() != strides or strides[0] < whole or strides[0] % 16 or d % 16
-            or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16 or k_cache.get_device() != device or v_cache.get_device() != device):
-        if pages:
-            raise ops.KernelError(f"pools with strides {strides} and {v_cache.stride()}: pages must be whole, 16-byte aligned and as far apart in both, "
-                                  f"head sizes multiples of 16, on cuda:{device}")
-    _need_all(device, torch.float32, k_scale=k_scale, v_scale=v_scale)
+    row = kv * d
+    if (strides[1:] != (row, d, 1) or v_cache.stride() != strides or strides[0] < page * row or strides[0] % 16 or d % 16
+            or (k_cache.data_ptr() | v_cache.data_ptr()) % 16 or k_cache.get_device() != device or v_cache.get_device() != device) and pages:
+        raise ops.KernelError(f"pools with strides {strides} and {v_cache.stride()}: pages must be whole, 16-byte aligned and as far apart in both, "
+                              f"head sizes multiples of 16, on cuda:{device}")
+    if not (_plain(k_scale, device, _F32) and _plain(v_scale, device, _F32)):
+        _refuse_plain(device, _F32, k_scale=k_scale, v_scale=v_scale)
     if k_scale.shape != (pages, kv) or v_scale.shape != (pages, kv):
         raise ops.KernelError(f"one scale per page and KV head: {tuple(k_scale.shape)}, {tuple(v_scale.shape)} for pools of {pages} pages and {kv} heads")
     return pages, page, kv, d, strides[0]
@@ -118,7 +128,8 @@ def store_kv8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: to
     device = k_cache.get_device()
     pages, page, kv, d, page_stride = _need_pools(device, k_cache, v_cache, k_scale, v_scale)
     n = slots.shape[0]
-    _need_all(device, _INT, slots=slots, status=status)
+    if not (_plain(slots, device, _INT) and _plain(status, device, _INT)):
+        _refuse_plain(device, _INT, slots=slots, status=status)
     if slots.dim() != 1 or k.shape != (n, kv, d) or v.shape != (n, kv, d) or k.dtype != v.dtype:
         raise ops.KernelError(f"k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} must be [{n}, {kv}, {d}] of one dtype for {n} slots")
     code = ops._dtype_code(k)
@@ -127,8 +138,11 @@ def store_kv8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: to
     k_stride, v_stride = _head_rows(k, "k", device), _head_rows(v, "v", device)
     if n == 0:
         return
+    ends = None if n <= KV8_FEW_TOKENS else slots.new_empty(2 * pages)
     ops._done(_core_lib().oxr_store_kv8(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k.data_ptr(), v.data_ptr(), k_stride,
-                                        v_stride, slots.data_ptr(), n, page_stride, pages, page, kv, d, code, status.data_ptr(), ops._stream()), "store_kv8")
+                                        v_stride, slots.data_ptr(), n, page_stride, pages, page, kv, d, code, ops._ptr(ends), status.data_ptr(), ops._stream()), "store_kv8")
+    if ends is not None:
+        ops.launch_count += 1
 
 
 @functools.lru_cache(maxsize=None)
@@ -182,14 +196,15 @@ def paged_attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         raise ops.KernelError(f"q {tuple(q.shape)} does not fit {kv} KV heads of {d}")
     tokens, heads = q.shape[0], q.shape[1]
     q_stride = _head_rows(q, "q", device)
-    _need_all(device, _INT, cu_q=cu_q, ctx_lens=ctx_lens, block_table=block_table, status=status)
+    if not (_plain(cu_q, device, _INT) and _plain(ctx_lens, device, _INT) and _plain(block_table, device, _INT) and _plain(status, device, _INT)):
+        _refuse_plain(device, _INT, cu_q=cu_q, ctx_lens=ctx_lens, block_table=block_table, status=status)
     n = ctx_lens.shape[0]
     if ctx_lens.dim() != 1 or cu_q.shape != (n + 1,) or block_table.dim() != 2 or block_table.shape[0] != n:
         raise ops.KernelError(f"cu_q {tuple(cu_q.shape)}, ctx_lens {tuple(ctx_lens.shape)} and block_table {tuple(block_table.shape)} are not of one batch")
     if window < 0 or max_q_len < 1:
         raise ops.KernelError(f"window {window}, max_q_len {max_q_len}")
     if out is None:
-        out = torch.empty((tokens, heads, d), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((tokens, heads, d))
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.get_device() != device or out.data_ptr() % 16:
         raise ops.KernelError(f"out {out.dtype} {tuple(out.shape)} must be a contiguous tensor like q {q.dtype} {tuple(q.shape)}")
     if n == 0 or tokens == 0:
@@ -212,7 +227,7 @@ def paged_attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     tiles = min(tokens, n * -(-longest // per_tile), n + tokens // per_tile) * kv * -(-group // heads_per_tile)
     seen = min(kv_len_bound, window + longest + 32) if window > 0 else kv_len_bound
     blocks = kv8_blocks(tiles, max(1, -(-seen // 32)), _kv8_room(d, code, rows))
-    scratch = torch.empty(8 * blocks * rows * (d + 2) + 32 * blocks, dtype=torch.float32, device=q.device)
+    scratch = k_scale.new_empty(8 * blocks * rows * (d + 2) + 32 * blocks)
     ops._done(lib.oxr_kv8_attention(*common, 1, longest, max_q_len, rows, blocks, scratch.data_ptr(), code, status.data_ptr(), ops._stream()), "paged_attention_kv8")
     ops.launch_count += 1
     return out
@@ -248,21 +263,24 @@ def step_pages(lengths: torch.Tensor, held: torch.Tensor, block_table: torch.Ten
     ``tokens`` tokens, the status word is set, nothing moves, and the arrays hold no token at all (slots -1, ``cu_q`` and ``ctx_lens`` 0)."""
     _here(block_table, "block_table")
     device = block_table.get_device()
-    _need_all(device, _INT, lengths=lengths, held=held, block_table=block_table, free_list=free_list, free_count=free_count, q_lens=q_lens, status=status)
+    if not (_plain(lengths, device, _INT) and _plain(held, device, _INT) and _plain(block_table, device, _INT) and _plain(free_list, device, _INT)
+            and _plain(free_count, device, _INT) and _plain(q_lens, device, _INT) and _plain(status, device, _INT)):
+        _refuse_plain(device, _INT, lengths=lengths, held=held, block_table=block_table, free_list=free_list, free_count=free_count, q_lens=q_lens, status=status)
     if block_table.dim() != 2:
         raise ops.KernelError(f"block_table must be [rows, pages], got {tuple(block_table.shape)}")
     rows, width = block_table.shape
-    if fresh is not None:
-        _need_all(device, _INT, fresh=fresh)
-    for name, t in (("lengths", lengths), ("held", held), ("q_lens", q_lens), ("fresh", fresh)):
-        if t is not None and t.shape != (rows,):
-            raise ops.KernelError(f"{name} {tuple(t.shape)}: one for each of {rows} rows")
+    one = (rows,)
+    if lengths.shape != one or held.shape != one or q_lens.shape != one or fresh is not None and not (fresh.shape == one and _plain(fresh, device, _INT)):
+        for name, t in (("lengths", lengths), ("held", held), ("q_lens", q_lens), ("fresh", fresh)):
+            if t is not None and t.shape != one:
+                raise ops.KernelError(f"{name} {tuple(t.shape)}: one for each of {rows} rows")
+        _refuse_plain(device, _INT, fresh=fresh)
     if free_count.numel() != 1 or free_list.dim() != 1:
         raise ops.KernelError(f"free_list {tuple(free_list.shape)} must be a row and free_count {tuple(free_count.shape)} one number")
     if page_size < 1 or tokens < 0 or rows > 8192:
         raise ops.KernelError(f"page size {page_size}, {tokens} tokens, {rows} rows: at most 8192 rows")
-    block = torch.empty(3 * tokens + 2 * rows + 1, dtype=_INT, device=block_table.device)
-    step = PageStep(*block.split((tokens, tokens, tokens, rows + 1, rows)))
+    block = block_table.new_empty(3 * tokens + 2 * rows + 1)
+    step = PageStep(*torch.split_with_sizes(block, (tokens, tokens, tokens, rows + 1, rows)))
     at = block.data_ptr()
     ops._done(_core_lib().oxr_step_pages(lengths.data_ptr(), held.data_ptr(), block_table.data_ptr(), free_list.data_ptr(), free_count.data_ptr(),
                                          q_lens.data_ptr(), ops._ptr(fresh), rows, width, int(page_size), free_list.shape[0], int(tokens), at,
