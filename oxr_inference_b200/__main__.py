@@ -37,7 +37,7 @@ def _generate(args: argparse.Namespace) -> int:
     settings = EngineSettings(kv_cache_gb=args.kv_gb, num_pages=args.num_pages, page_size=args.page_size,
                               max_running=args.max_running, max_waiting=args.max_waiting, max_step_tokens=args.max_step_tokens,
                               prefill_chunk=args.prefill_chunk, max_positions=args.max_positions,
-                              cuda_graphs=not args.no_cuda_graphs, dtype=args.dtype)
+                              cuda_graphs=not args.no_cuda_graphs, dtype=args.dtype, kv_cache_dtype=args.kv_cache_dtype)
     engine = Engine(args.model, settings)
     params = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, seed=args.seed,
                             repetition_penalty=args.repetition_penalty, ignore_eos=args.ignore_eos)
@@ -84,6 +84,7 @@ def main(argv: list[str] | None = None) -> int:
     g.add_argument("--repetition-penalty", type=float, default=1.0)
     g.add_argument("--ignore-eos", action="store_true")
     g.add_argument("--dtype", choices=("bfloat16", "float32"), default="bfloat16")
+    g.add_argument("--kv-cache-dtype", choices=("auto", "e4m3"), default="auto", help="e4m3: keys and values in 8 bits")
     g.add_argument("--kv-gb", type=float, default=16.0, help="device memory for the paged cache")
     g.add_argument("--num-pages", type=int, default=None, help="pages per cache group (overrides --kv-gb)")
     g.add_argument("--page-size", type=int, default=16)

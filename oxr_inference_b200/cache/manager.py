@@ -21,6 +21,7 @@ from oxr_inference_b200.cache.pages import PagePool
 from oxr_inference_b200.cache.plan import CachePlan
 from oxr_inference_b200.parts.base import GroupView, LayerCache, StepContext
 
+EIGHT_BIT = torch.float8_e4m3fn
 RELEASED = -1
 """Block-table entry of a page that a window has passed."""
 
@@ -81,10 +82,20 @@ class CacheManager:
         self.device, self.dtype = device, dtype
         self.k_pools: list[torch.Tensor] = []
         self.v_pools: list[torch.Tensor] = []
+        self.scales: list[tuple[torch.Tensor | None, torch.Tensor | None]] = []
+        """Per group of 8-bit keys and values: their scales (keys, values); a page needs no preparation when it goes to another request, storing
+        its first slot begins its scales anew."""
         self.states: list[torch.Tensor] = []
         if device is not None:
             for g in plan.groups:
                 shape = (g.num_layers, num_pages, page_size, g.need.num_kv_heads)
+                if g.need.eight_bit:
+                    self.k_pools.append(torch.zeros((*shape, g.need.head_dim), dtype=torch.uint8, device=device).view(EIGHT_BIT))
+                    self.v_pools.append(torch.zeros((*shape, g.need.v_dim), dtype=torch.uint8, device=device).view(EIGHT_BIT))
+                    scales = (g.num_layers, num_pages, g.need.num_kv_heads)
+                    self.scales.append((torch.zeros(scales, device=device), torch.zeros(scales, device=device)))
+                    continue
+                self.scales.append((None, None))
                 self.k_pools.append(torch.zeros((*shape, g.need.head_dim), dtype=dtype, device=device))
                 # a group whose values are read from its key rows has no value pool
                 self.v_pools.append(torch.zeros((*shape, g.need.v_dim), dtype=dtype, device=device) if g.need.v_dim > 0 else None)
@@ -95,6 +106,7 @@ class CacheManager:
         if device is not None and torch.device(device).type == "cuda":
             from oxr_inference_b200 import ops
 
+            ops.warm_up_kv8(tuple({g.need.head_dim for g in plan.groups if g.need.eight_bit}))
             # TMA maps serve the kernels of plain grouped-query attention: keys and values of one size, causal or windowed
             self.kv_maps = [ops.make_kv_maps(k, v, page_size) if (g.need.value_dim is None and g.need.chunk == 0) else None
                             for g, k, v in zip(plan.groups, self.k_pools, self.v_pools)]
@@ -107,9 +119,10 @@ class CacheManager:
     # ---- sizes
     @staticmethod
     def bytes_per_page(plan: CachePlan, page_size: int, dtype: torch.dtype) -> int:
-        """Bytes of one page id over all groups and layers (oxr_runtime/kv_cache.py:34-37)."""
+        """Bytes of one page id over all groups and layers (oxr_runtime/kv_cache.py:34-37); 8-bit groups have two fp32 scales per KV head beside their codes."""
         element = torch.empty((), dtype=dtype).element_size()
-        return sum(g.num_layers * page_size * g.need.num_kv_heads * (g.need.head_dim + g.need.v_dim) * element for g in plan.groups)
+        return sum(g.num_layers * g.need.num_kv_heads * (page_size * (g.need.head_dim + g.need.v_dim) * (1 if g.need.eight_bit else element) + (8 if g.need.eight_bit else 0))
+                   for g in plan.groups)
 
     @property
     def free_pages(self) -> int:
@@ -268,4 +281,5 @@ class CacheManager:
     def group_view(self, group: int, block_table: torch.Tensor, slots: torch.Tensor) -> GroupView:
         return GroupView(self.page_size, self.k_pools[group] if self.k_pools else None,
                          self.v_pools[group] if self.v_pools else None, block_table, slots,
-                         self.kv_maps[group] if self.k_pools else None, self.long_maps[group] if self.k_pools else None)
+                         self.kv_maps[group] if self.k_pools else None, self.long_maps[group] if self.k_pools else None,
+                         *(self.scales[group] if self.k_pools else ()))

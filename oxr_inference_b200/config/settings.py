@@ -32,6 +32,9 @@ class EngineSettings:
     """Replay decode-only steps from CUDA graphs (oxr_runtime/decode_graph.py)."""
     dtype: str = "bfloat16"
     """``bfloat16``: the serving kernels; ``float32``: every operation in true 32-bit."""
+    kv_cache_dtype: str = "auto"
+    """``auto``: keys and values are cached in ``dtype``; ``e4m3``: in 8 bits with a scale for each page and KV head, in the layers of plain grouped-query
+    attention (half the cache memory of bfloat16 and half the bytes that a decode step reads of it)."""
     profile: bool = False
     """Keep per-stage timers and a per-step log in ``Engine.profile`` (also switched on by ``OXR_PROFILE=1`` in the
     environment, the reference's switch, oxr_runtime/engine.py:62-63)."""
@@ -42,6 +45,8 @@ class EngineSettings:
     def __post_init__(self) -> None:
         if self.dtype not in ("bfloat16", "float32"):
             raise ValueError(f"dtype must be 'bfloat16' or 'float32', got {self.dtype!r}")
+        if self.kv_cache_dtype not in ("auto", "e4m3"):
+            raise ValueError(f"kv_cache_dtype must be 'auto' or 'e4m3', got {self.kv_cache_dtype!r}")
         if self.page_size <= 0:
             raise ValueError("page_size must be positive")
         if self.max_step_tokens < 1 or self.prefill_chunk < 1 or self.max_running < 1:

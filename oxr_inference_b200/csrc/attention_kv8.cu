@@ -694,64 +694,67 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
     if (lane == 0) left.cuts[me] = cut;
 }
 
-// Joins the pieces of the tiles that lie in more than one warp's stretch. Block b takes the tile that stretch b ends in, if it began there. A
-// thread has four entries of a row; where the rows leave threads over, they take the pieces in turn.
-constexpr int JOIN_THREADS = 256;
+// Joins the pieces of the tiles that lie in more than one warp's stretch. A block looks at some of the stretches and, of each that ends in a tile
+// which began in it, takes four rows of the tile. A thread has four entries of a row; where the rows leave threads over, they take the pieces in turn.
+constexpr int JOIN_THREADS = 256, JOIN_ROWS = 4, JOIN_BLOCKS = 592;
 template <typename T, int NQ>
-__global__ void __launch_bounds__(JOIN_THREADS) attn_kv8_join_kernel(T* __restrict__ out, const Pieces left, const int H, const int heads_per_tile) {
+__global__ void __launch_bounds__(JOIN_THREADS) attn_kv8_join_kernel(T* __restrict__ out, const Pieces left, const int warps, const int H, const int heads_per_tile) {
     constexpr int ROWS = 8 * NQ, WORDS = D / 4;
     __shared__ float4 sums[JOIN_THREADS];
     __shared__ float2 ml[JOIN_THREADS];
     pdl_wait();
     pdl_trigger();
-    const int first = blockIdx.x;
-    const int4 c0 = __ldcg(reinterpret_cast<const int4*>(left.cuts + first)), c1 = __ldcg(reinterpret_cast<const int4*>(left.cuts + first) + 1);
-    const Cut cut = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, {0, 0}};
-    if (cut.last < 0) return;
-    const float unscale = exp2_of((float)cut.base_exp);
-    const int all = cut.rows * WORDS;
-    int ways = 1;      // threads that share an entry's pieces
-    while (ways * 2 * all <= JOIN_THREADS) ways *= 2;
-    for (int x0 = 0; x0 < all; x0 += JOIN_THREADS) {
-        const int x = ways > 1 ? threadIdx.x % all : x0 + threadIdx.x, way = ways > 1 ? threadIdx.x / all : 0;
-        const int r = x / WORDS, d = x % WORDS * 4;
-        const bool there = x < all && way < ways;
-        float top = -INFINITY, total = 0.f;
-        float4 v[1] = {make_float4(0.f, 0.f, 0.f, 0.f)};
-        if (there) {
-            for (int w0 = first + way; w0 <= cut.last; w0 += 8 * ways) {     // eight pieces at a time
-                float2 y[8];
-                float4 u[8][1];
+    const int lane = threadIdx.x & 31, r0 = (int)blockIdx.y * JOIN_ROWS;
+    for (int w0 = blockIdx.x; w0 < warps; w0 += 32 * (int)gridDim.x) {
+        const int mine = w0 + lane * (int)gridDim.x;
+        for (unsigned valid = __ballot_sync(0xffffffffu, mine < warps && __ldcg(&left.cuts[mine < warps ? mine : 0].last) >= 0); valid; valid &= valid - 1) {
+            const int first = w0 + (__ffs(valid) - 1) * (int)gridDim.x;       // the same in every warp
+            const int4 c0 = __ldcg(reinterpret_cast<const int4*>(left.cuts + first)), c1 = __ldcg(reinterpret_cast<const int4*>(left.cuts + first) + 1);
+            const Cut cut = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, {0, 0}};
+            if (r0 >= cut.rows) continue;
+            const int all = min(JOIN_ROWS, cut.rows - r0) * WORDS;
+            int ways = 1;      // threads that share an entry's pieces
+            while (ways * 2 * all <= JOIN_THREADS) ways *= 2;
+            const int x = threadIdx.x % all, way = threadIdx.x / all, r = r0 + x / WORDS, d = x % WORDS * 4;
+            float top = -INFINITY, total = 0.f;
+            float4 v[1] = {make_float4(0.f, 0.f, 0.f, 0.f)};
+            if (way < ways) {
+                for (int p0 = first + way; p0 <= cut.last; p0 += 8 * ways) {     // eight pieces at a time
+                    float2 y[8];
+                    float4 u[8][1];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int w = w0 + k * ways;
-                    const size_t at = ((size_t)2 * w + (w == first ? 1 : 0)) * ROWS + r;
-                    y[k] = w <= cut.last ? __ldcg(left.ml + at) : make_float2(-INFINITY, 0.f);
-                    u[k][0] = w <= cut.last ? __ldcg(reinterpret_cast<const float4*>(left.sums + at * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int k = 0; k < 8; ++k) {
+                        const int w = p0 + k * ways;
+                        const size_t at = ((size_t)2 * w + (w == first ? 1 : 0)) * ROWS + r;
+                        y[k] = w <= cut.last ? __ldcg(left.ml + at) : make_float2(-INFINITY, 0.f);
+                        u[k][0] = w <= cut.last ? __ldcg(reinterpret_cast<const float4*>(left.sums + at * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) add_piece<1>(top, total, v, y[k], u[k]);
                 }
-#pragma unroll
-                for (int k = 0; k < 8; ++k) add_piece<1>(top, total, v, y[k], u[k]);
             }
-        }
-        if (ways > 1) {
-            sums[threadIdx.x] = v[0];
-            ml[threadIdx.x] = make_float2(top, total);
-            __syncthreads();
-            if (there && way == 0)
-                for (int k = 1; k < ways; ++k) {
-                    const float4 u[1] = {sums[k * all + x]};
-                    add_piece<1>(top, total, v, ml[k * all + x], u);
-                }
-        }
-        const int head = r % heads_per_tile;
-        if (there && way == 0 && head < cut.heads) {
-            const float f = (1.f / P_FACTOR) / total;
-            float4 z = make_float4(v[0].x * f * unscale, v[0].y * f * unscale, v[0].z * f * unscale, v[0].w * f * unscale);
-            if (total == 0.f) z = make_float4(0.f, 0.f, 0.f, 0.f);
-            store4(out + ((size_t)(cut.token + r / heads_per_tile) * H + cut.head + head) * D + d, z);
+            if (ways > 1) {
+                sums[threadIdx.x] = v[0];
+                ml[threadIdx.x] = make_float2(top, total);
+                __syncthreads();
+                if (way == 0)
+                    for (int k = 1; k < ways; ++k) {
+                        const float4 u[1] = {sums[k * all + x]};
+                        add_piece<1>(top, total, v, ml[k * all + x], u);
+                    }
+                __syncthreads();
+            }
+            const int head = r % heads_per_tile;
+            if (way == 0 && head < cut.heads) {
+                const float f = (1.f / P_FACTOR) / total, unscale = exp2_of((float)cut.base_exp);
+                float4 z = make_float4(v[0].x * f * unscale, v[0].y * f * unscale, v[0].z * f * unscale, v[0].w * f * unscale);
+                if (total == 0.f) z = make_float4(0.f, 0.f, 0.f, 0.f);
+                store4(out + ((size_t)(cut.token + r / heads_per_tile) * H + cut.head + head) * D + d, z);
+            }
         }
     }
 }
+static_assert(JOIN_ROWS * D / 4 <= JOIN_THREADS, "a thread for every entry of the rows that a block takes");
 
 // A pool of pages seen as boxes of `piece` keys x PW bytes of one KV head.
 bool make_map(CUtensorMap* map, const void* base, const Kv8Args& a, int piece) {
@@ -791,7 +794,8 @@ int launch(void* out, const void* q, const Kv8Args& a, int blocks, float* scratc
     const dim3 grid(blocks), threads(THREADS);
     if (tma) oxr_launch(attn_kv8_kernel<T, true, NQ>, grid, threads, Shape<T, NQ>::SMEM, stream, true, (T*)out, (const T*)q, map_k, map_v, piece_shift, a, left);
     else oxr_launch(attn_kv8_kernel<T, false, NQ>, grid, threads, Shape<T, NQ>::SMEM, stream, true, (T*)out, (const T*)q, map_k, map_v, piece_shift, a, left);
-    if (warps > 1) oxr_launch(attn_kv8_join_kernel<T, NQ>, dim3(warps - 1), dim3(JOIN_THREADS), 0, stream, true, (T*)out, left, a.H, a.heads_per_tile);
+    const dim3 join(warps < JOIN_BLOCKS ? warps : JOIN_BLOCKS, 8 * NQ / JOIN_ROWS);
+    oxr_launch(attn_kv8_join_kernel<T, NQ>, join, dim3(JOIN_THREADS), 0, stream, true, (T*)out, left, warps, a.H, a.heads_per_tile);
     return oxr_launch_status();
 }
 }  // namespace

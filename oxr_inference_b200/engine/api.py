@@ -71,7 +71,7 @@ class Engine:
             raw, generation = dict(random_config), None
         shapes = tensor_shapes(model_dir) if model_dir is not None and resolve_architecture(raw).shapes_matter else None
         model, self.config = ModelRunner.build_model(raw, generation, dtype=s.dtype, device=device, max_positions=s.max_positions,
-                                                      page_size=s.page_size, shapes=shapes)
+                                                      page_size=s.page_size, kv_cache_dtype=s.kv_cache_dtype, shapes=shapes)
         if model_dir is not None:
             load_weights(model, model_dir)
         else:

@@ -51,32 +51,36 @@ class ModelRunner:
     @staticmethod
     def build_model(raw_config: Mapping[str, Any], generation: Mapping[str, Any] | None, *, dtype: str,
                     device: str | torch.device = "cuda", max_positions: int | None = None, page_size: int = 16,
-                    shapes: Mapping[str, tuple[int, ...]] | None = None):
+                    kv_cache_dtype: str = "auto", shapes: Mapping[str, tuple[int, ...]] | None = None):
         """``shapes``: the checkpoint's tensor shapes, for designs that leave a size to them (``Architecture.shapes_matter``)."""
         dev = require_cuda(device)
         arch = resolve_architecture(raw_config)
         config = arch.config_from_dict(raw_config, generation)
         spec = arch.spec_for(config, shapes)
         runtime = Runtime(device=dev, dtype=DTYPES[dtype], max_positions=max_positions or spec.max_positions,
-                          status=ops.new_status(dev), page_size=page_size)
-        return DecoderModel(spec, runtime), config
+                          status=ops.new_status(dev), page_size=page_size, kv_dtype=kv_cache_dtype)
+        model = DecoderModel(spec, runtime)
+        if kv_cache_dtype != "auto" and not any(g.need.eight_bit for g in model.cache_plan.groups):
+            raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r}: no layer of this model keeps keys and values that could be held in 8 bits")
+        return model, config
 
     @classmethod
     def from_folder(cls, model_dir: str | Path, *, dtype: str, page_size: int, num_pages: int, max_requests: int,
-                    device: str | torch.device = "cuda", max_positions: int | None = None) -> "ModelRunner":
+                    device: str | torch.device = "cuda", max_positions: int | None = None, kv_cache_dtype: str = "auto") -> "ModelRunner":
         raw, generation = read_config_json(model_dir)
         arch = resolve_architecture(raw)
         model, config = cls.build_model(raw, generation, dtype=dtype, device=device, max_positions=max_positions, page_size=page_size,
-                                        shapes=tensor_shapes(model_dir) if arch.shapes_matter else None)
+                                        kv_cache_dtype=kv_cache_dtype, shapes=tensor_shapes(model_dir) if arch.shapes_matter else None)
         load_weights(model, model_dir)
         return cls(model, config, page_size=page_size, num_pages=num_pages, max_requests=max_requests)
 
     @classmethod
     def from_config(cls, raw_config: Mapping[str, Any], seed: int, *, dtype: str, page_size: int, num_pages: int,
                     max_requests: int, device: str | torch.device = "cuda", max_positions: int | None = None,
-                    std: float = 0.02, norm_std: float = 0.1) -> "ModelRunner":
+                    std: float = 0.02, norm_std: float = 0.1, kv_cache_dtype: str = "auto") -> "ModelRunner":
         """Random weights drawn on the device (no file)."""
-        model, config = cls.build_model(raw_config, None, dtype=dtype, device=device, max_positions=max_positions, page_size=page_size)
+        model, config = cls.build_model(raw_config, None, dtype=dtype, device=device, max_positions=max_positions, page_size=page_size,
+                                        kv_cache_dtype=kv_cache_dtype)
         fill_random(model, seed, std=std, norm_std=norm_std)
         return cls(model, config, page_size=page_size, num_pages=num_pages, max_requests=max_requests)
 

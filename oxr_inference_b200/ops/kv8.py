@@ -63,6 +63,14 @@ def _core_lib():
     return _core
 
 
+def warm_up_kv8(head_dims: tuple[int, ...]) -> None:
+    """Build and load the libraries of an 8-bit cache with these head sizes, before the first step."""
+    if head_dims:
+        _core_lib()
+    for d in head_dims:
+        _kv8_lib(d)
+
+
 def _here(t: torch.Tensor, name: str) -> None:
     """The launch goes to the current device's current stream, so the tensors have to be there."""
     if not t.is_cuda:
@@ -159,22 +167,30 @@ def kv8_blocks(tiles: int, key_blocks: int, room: int) -> int:
 
 KV8_PROMPT_ROWS = 256
 """Rows of a tile of the tcgen05 kernel for long portions."""
-KV8_PROMPT_TILES = 24
-"""From how many such tiles on that kernel takes a step's portions of more than ``ops.SHORT_MAX_TOKENS`` tokens. A tile walks over its keys alone, so a few of them
-leave most of the GPU idle. Measured on a B200 (32 / 8 heads of 128), that kernel against the split-key one: 8 tiles on 4,096 keys 87 and 49 us, 16 on 8,192 keys 160
-and 125, 32 on 4,096 keys 88 and 129, 64 on 512 keys 24 and 52."""
 
 
-def kv8_prompt_tiles(tokens: int, max_q_len: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, scale: float) -> int:
-    """Tiles that the tcgen05 kernel would have to do for one KV head's query heads, about; 0 where the split-key kernel does the whole step: other types and
-    sizes, a scale that is not positive (the row's maximum is scaled, not each score), short portions, or too few tiles."""
-    if dtype != torch.bfloat16 or head_dim > 128 or not scale > 0 or max_q_len <= ops.SHORT_MAX_TOKENS:
-        return 0
+def kv8_prompt_takes(max_q_len: int, head_dim: int, dtype: torch.dtype, scale: float) -> bool:
+    """Whether the tcgen05 kernel can take the longer portions of a step: bfloat16 queries, head sizes up to 128, a positive scale (it scales a row's maximum,
+    not each score)."""
+    return dtype == torch.bfloat16 and head_dim <= 128 and scale > 0 and max_q_len > ops.SHORT_MAX_TOKENS
+
+
+def kv8_prompt_pays(requests: int, tokens: int, max_q_len: int, num_heads: int, num_kv_heads: int, head_dim: int, seen: int) -> bool:
+    """Whether it is also the faster one for portions of more than ``ops.SHORT_MAX_TOKENS`` tokens that see up to ``seen`` keys. Its tiles (256 rows) walk over their
+    keys alone, 2.5 us for each 128 of them, so that a few tiles leave most of the GPU idle; the split-key kernel deals all work out evenly but
+    needs 1.8 ns for each 16 rows x 32 keys x 128 entries. Measured on a B200 (32 / 8 heads of 128), this one against that one: 64 tokens on 4,096 keys 87
+    and 49 us, 128 on 8,192 160 and 125, 256 on 4,096 88 and 129, 512 on 512 24 and 52, 16 requests of 16 tokens on 2,048 51 and 76, 2,048 on 4,096 142 and 890."""
     group = num_heads // num_kv_heads
-    heads_per_tile = min(group, KV8_PROMPT_ROWS)
-    per_tile = KV8_PROMPT_ROWS // heads_per_tile
-    tiles = max(-(-max_q_len // per_tile), tokens // per_tile)
-    return tiles if tiles * num_kv_heads * -(-group // heads_per_tile) >= KV8_PROMPT_TILES else 0
+
+    def cut(rows: int) -> tuple[int, int]:      # tokens of a tile, tiles that the heads of all KV heads make
+        heads = min(group, rows)
+        return rows // heads, num_kv_heads * -(-group // heads)
+
+    per_tile, across = cut(KV8_PROMPT_ROWS)
+    tiles = max(-(-max_q_len // per_tile), tokens // per_tile, requests if tokens > ops.SHORT_MAX_TOKENS * requests else 1) * across
+    short_per_tile, short_across = cut(16)
+    items = tokens / short_per_tile * short_across * -(-seen // 32) * head_dim / 128
+    return 15 + 2.5 * -(-seen // 128) * max(1.0, tiles / 148) < 12 + 0.0018 * items
 
 
 def paged_attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, *,
@@ -214,7 +230,8 @@ def paged_attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     common = (out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), cu_q.data_ptr(), ctx_lens.data_ptr(),
               block_table.data_ptr(), n, tokens, block_table.shape[1], page, page_stride, pages, heads, kv, q_stride, float(scale), int(window))
     longest = max_q_len = int(max_q_len)
-    if kv8_prompt_tiles(tokens, max_q_len, heads, kv, d, q.dtype, scale):
+    seen = max(1, min(kv_len_bound, window + max_q_len) if window > 0 else kv_len_bound)
+    if kv8_prompt_takes(max_q_len, d, q.dtype, scale) and kv8_prompt_pays(n, tokens, max_q_len, heads, kv, d, seen):
         fewest = ops.SHORT_MAX_TOKENS + 1 if n > 1 else 1      # a request alone goes there whatever it brings
         tiles = min(tokens, min(n, tokens // fewest) + tokens // (KV8_PROMPT_ROWS // min(group, KV8_PROMPT_ROWS)))
         ops._done(lib.oxr_kv8_prompt_attention(*common, fewest, max_q_len, max_q_len, tiles, status.data_ptr(), ops._stream()), "paged_attention_kv8 (prompts)")

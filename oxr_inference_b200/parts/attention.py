@@ -55,12 +55,14 @@ class GroupedQueryAttention(Mixer):
             raise KeyError(name)
 
     def cache_need(self) -> PagedKVNeed:
-        return PagedKVNeed(self.KV, self.D, self.window)
+        return PagedKVNeed(self.KV, self.D, self.window, eight_bit=self.runtime.kv_dtype == "e4m3")
 
     def kernel_head_dims(self) -> tuple[int, ...]:
-        return (self.D,)
+        return () if self.runtime.kv_dtype == "e4m3" else (self.D,)     # the 8-bit cache's kernels are loaded with its pools
 
     def tile_specs(self) -> list[tuple[int, int, int]]:
+        if self.runtime.kv_dtype == "e4m3":
+            return []       # those kernels find their tiles themselves
         return ops.attention_tile_specs(self.H, self.KV, self.D, self.runtime.dtype, self.runtime.page_size)
 
     accepts_lazy_input = True   # h goes into the q|k|v projection and nowhere else
@@ -76,9 +78,12 @@ class GroupedQueryAttention(Mixer):
         group = cache.group
         k_pool, v_pool = group.k_pool[cache.layer_in_group], group.v_pool[cache.layer_in_group]
         qkv = self.qkv(h)
-        if qkv.dtype != k_pool.dtype:  # weights kept in 32-bit under 16-bit activations
-            qkv = ops.cast(qkv, k_pool.dtype)
+        dtype = k_pool.dtype if group.k_scale is None else self.runtime.dtype
+        if qkv.dtype != dtype:  # weights kept in 32-bit under 16-bit activations
+            qkv = ops.cast(qkv, dtype)
         cos, sin = self.position.tables() if self.position is not None else (None, None)
+        if group.k_scale is not None:
+            return self._attend_8bit(qkv, cos, sin, ctx, cache).view(ctx.n_tokens, self.H * self.D)
         if ctx.single_tokens and ops.attention_takes_projections(self.D, qkv.dtype, group.page_size, group.kv_maps, requests=ctx.n_requests,
                                                                  num_heads=self.H, num_kv_heads=self.KV, kv_len_bound=ctx.kv_len_bound,
                                                                  uneven=ctx.uneven):
@@ -97,3 +102,18 @@ class GroupedQueryAttention(Mixer):
                                 window=self.window, kv_len_bound=ctx.kv_len_bound, status=ctx.status,
                                 kv_maps=group.kv_maps, layer_in_pool=cache.layer_in_group, uneven=ctx.uneven)
         return o.view(ctx.n_tokens, self.H * self.D)
+
+    def _attend_8bit(self, qkv: torch.Tensor, cos: torch.Tensor | None, sin: torch.Tensor | None, ctx: StepContext, cache: LayerCache) -> torch.Tensor:
+        """The same over a cache of 8-bit keys and values: the step's own go through a buffer of their own, one row a token, on their way into it."""
+        group, layer = cache.group, cache.layer_in_group
+        rows = ctx.shared.get("token_rows")
+        if rows is None:
+            rows = ctx.shared["token_rows"] = torch.arange(ctx.n_tokens, dtype=torch.int32, device=qkv.device)
+        new = qkv.new_empty((2, ctx.n_tokens, self.KV, self.D))
+        q = ops.qk_norm_rope_store(qkv, self.q_norm, self.k_norm, cos, sin, ctx.positions, rows if cache.store else ctx.no_store_slots, new[0], new[1],
+                                   self.H, self.KV, self.D, self.eps, ctx.status)
+        pools = (group.k_pool[layer], group.v_pool[layer], group.k_scale[layer], group.v_scale[layer])
+        if cache.store:
+            ops.store_kv8(new[0], new[1], group.slots, *pools, ctx.status)
+        return ops.paged_attention_kv8(q, *pools, cu_q=ctx.cu_q, ctx_lens=ctx.ctx_lens, block_table=group.block_table, scale=self.scale, window=self.window,
+                                       max_q_len=max(ctx.q_lens), kv_len_bound=ctx.kv_len_bound, status=ctx.status)

@@ -47,6 +47,8 @@ class Runtime:
     """Device status word that kernels write their first error to (see ``ops.check_status``)."""
     page_size: int = 16
     """Tokens per cache page (an engine setting): kernels that read the cache may plan their tiles by it."""
+    kv_dtype: str = "auto"
+    """What mixers that can choose keep their keys and values in: ``auto``: ``dtype``; ``e4m3``: 8 bits with a scale per page and KV head."""
 
     def store_dtype(self, info: ParamInfo, stored: torch.dtype) -> torch.dtype:
         if info.role == "vector" or self.dtype == torch.float32:
@@ -87,6 +89,8 @@ class PagedKVNeed:
     query are released."""
     keep_first: int = 0
     """With a window: the request's first ``keep_first`` keys stay visible to every later query, so the pages that hold them are never released."""
+    eight_bit: bool = False
+    """Keys and values are e4m3 codes with fp32 scales per page and KV head (``ops.store_kv8``)."""
 
     @property
     def v_dim(self) -> int:
@@ -118,6 +122,9 @@ class GroupView:
     """TMA tensor maps over the pools (``ops.make_kv_maps``), when the sizes allow them."""
     long_maps: object | None = None
     """The same for mixers whose masks, or whose keys that are the values, keep them off ``kv_maps`` (``ops.masked_tile_specs``)."""
+    k_scale: torch.Tensor | None = None
+    """[layers of the group, pages, KV] fp32 for a group of 8-bit keys and values (``PagedKVNeed.eight_bit``)"""
+    v_scale: torch.Tensor | None = None
 
 
 @dataclass

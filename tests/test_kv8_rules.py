@@ -114,13 +114,19 @@ def test_bad_tables(on_cpu):
         ops.step_pages(many, many, torch.zeros((8193, 1), dtype=INT), good["free_list"], good["free_count"], many, page_size=16, tokens=1, status=status())
 
 
-def test_who_does_a_step():
+def test_who_can_do_a_step():
     bf16 = torch.bfloat16
-    assert kv8.kv8_prompt_tiles(2048, 2048, 32, 8, 128, bf16, 0.1) == 32
-    for tokens, most, heads, kv, d, dtype, scale in ((2048, 2048, 32, 8, 128, torch.float32, 0.1), (2048, 2048, 32, 8, 256, bf16, 0.1), (2048, 2048, 32, 8, 128, bf16, 0.0),
-                                                     (2048, 2048, 32, 8, 128, bf16, -0.1), (4096, 8, 32, 8, 128, bf16, 0.1), (64, 64, 32, 8, 128, bf16, 0.1)):
-        assert kv8.kv8_prompt_tiles(tokens, most, heads, kv, d, dtype, scale) == 0
-    assert kv8.kv8_prompt_tiles(1024, 16, 32, 8, 128, bf16, 0.1) == 16       # many short portions
+    assert kv8.kv8_prompt_takes(2048, 128, bf16, 0.1) and kv8.kv8_prompt_takes(9, 16, bf16, 1e-9)
+    for most, d, dtype, scale in ((2048, 128, torch.float32, 0.1), (2048, 256, bf16, 0.1), (2048, 128, bf16, 0.0), (2048, 128, bf16, -0.1), (8, 128, bf16, 0.1)):
+        assert not kv8.kv8_prompt_takes(most, d, dtype, scale)
+
+
+@pytest.mark.parametrize("requests,q,seen,heads,kv,d,pays", [(1, 2048, 4096, 32, 8, 128, True), (1, 64, 4096, 32, 8, 128, False), (1, 128, 8192, 32, 8, 128, False),
+                                                            (1, 256, 4096, 32, 8, 128, True), (16, 16, 2048, 32, 8, 128, True), (1, 512, 512, 32, 8, 128, True),
+                                                            (1, 256, 4096, 8, 8, 128, False), (1, 2048, 8192, 8, 1, 128, True), (16, 25, 552, 16, 2, 64, False)])
+def test_who_is_faster(requests, q, seen, heads, kv, d, pays):
+    """The sides that were measured to be."""
+    assert kv8.kv8_prompt_pays(requests, requests * q, q, heads, kv, d, seen) == pays
 
 
 def test_blocks():
