@@ -695,8 +695,8 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
 }
 
 // Joins the pieces of the tiles that lie in more than one warp's stretch. A block looks at some of the stretches and, of each that ends in a tile
-// which began in it, takes four rows of the tile. A thread has four entries of a row; where the rows leave threads over, they take the pieces in turn.
-constexpr int JOIN_THREADS = 256, JOIN_ROWS = 4, JOIN_BLOCKS = 592;
+// which began in it, takes eight rows of the tile. A thread has four entries of a row; where the rows leave threads over, they take the pieces in turn.
+constexpr int JOIN_THREADS = 256, JOIN_ROWS = D <= 128 ? 8 : 4, JOIN_BLOCKS = 592;
 template <typename T, int NQ>
 __global__ void __launch_bounds__(JOIN_THREADS) attn_kv8_join_kernel(T* __restrict__ out, const Pieces left, const int warps, const int H, const int heads_per_tile) {
     constexpr int ROWS = 8 * NQ, WORDS = D / 4;
@@ -807,20 +807,11 @@ OXR_API int oxr_kv8_blocks_per_sm(int dtype, int tile_rows) {
     return tile_rows == 8 ? (dtype == 0 ? Shape<float, 1>::BLOCKS : Shape<__nv_bfloat16, 1>::BLOCKS) : (dtype == 0 ? Shape<float, 2>::BLOCKS : Shape<__nv_bfloat16, 2>::BLOCKS);
 }
 
-// q [n_tokens, H, D] (tokens q_stride entries apart), out [n_tokens, H, D]; K and V pools of e4m3 codes with pages page_stride bytes apart and each
-// page [page_size, KV, D]; scales [num_pages, KV]; cu_q [n + 1], ctx_lens [n], block_table [n, table_width]. Requests of min_q .. max_q new
-// tokens are worked on; `any_q` is the most that any request may bring. dtype 0: fp32, 1: bf16; tiles of `tile_rows` (8 or 16) rows. `blocks` of four warps share
-// the work; `scratch` holds 8 * blocks * tile_rows * (D + 2) + 32 * blocks words.
-OXR_API int oxr_kv8_attention(void* out, const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, const int* cu_q,
-                              const int* ctx_lens, const int* block_table, int n, int n_tokens, int table_width, int page_size, long long page_stride,
-                              int num_pages, int H, int KV, long long q_stride, float scale, int window, int min_q, int max_q, int any_q, int tile_rows, int blocks,
-                              float* scratch, int dtype, int* status, cudaStream_t stream) {
-    if (n < 0 || n_tokens < 0 || KV <= 0 || H <= 0 || H % KV || page_size <= 0 || table_width < 0 || num_pages < 0 || window < 0) return OXR_BAD_ARGUMENT;
-    if (blocks < 1 || blocks > 65536 || scratch == nullptr || (dtype != 0 && dtype != 1) || any_q < 1 || min_q < 1 || (tile_rows != 8 && tile_rows != 16))
-        return OXR_BAD_ARGUMENT;
-    if (n == 0 || n_tokens == 0) return 0;
-    const Kv8Args a = kv8_args(k_cache, v_cache, k_scale, v_scale, cu_q, ctx_lens, block_table, n, n_tokens, table_width, page_size, page_stride, num_pages, H,
-                               KV, q_stride, scale, window, min_q, max_q, any_q, tile_rows, status);
-    if (tile_rows == 8) return dtype == 0 ? launch<float, 1>(out, q, a, blocks, scratch, stream) : launch<__nv_bfloat16, 1>(out, q, a, blocks, scratch, stream);
-    return dtype == 0 ? launch<float, 2>(out, q, a, blocks, scratch, stream) : launch<__nv_bfloat16, 2>(out, q, a, blocks, scratch, stream);
+OXR_API int oxr_kv8_attention(const Kv8Call* c) {
+    if (!kv8_call_ok(*c) || c->blocks < 1 || c->blocks > 65536 || c->scratch == nullptr || (c->tile_rows != 8 && c->tile_rows != 16)) return OXR_BAD_ARGUMENT;
+    if (c->n == 0 || c->n_tokens == 0) return 0;
+    const Kv8Args a = kv8_args(*c, c->tile_rows);
+    if (c->tile_rows == 8)
+        return c->dtype == 0 ? launch<float, 1>(c->out, c->q, a, c->blocks, c->scratch, c->stream) : launch<__nv_bfloat16, 1>(c->out, c->q, a, c->blocks, c->scratch, c->stream);
+    return c->dtype == 0 ? launch<float, 2>(c->out, c->q, a, c->blocks, c->scratch, c->stream) : launch<__nv_bfloat16, 2>(c->out, c->q, a, c->blocks, c->scratch, c->stream);
 }

@@ -35,39 +35,64 @@ struct Kv8Args {
     __device__ __forceinline__ int in_page(int key) const { return page_shift >= 0 ? key & (page_size - 1) : key % page_size; }
 };
 
-inline Kv8Args kv8_args(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, const int* cu_q, const int* ctx_lens,
-                        const int* block_table, int n, int n_tokens, int table_width, int page_size, long long page_stride, int num_pages, int H, int KV,
-                        long long q_stride, float scale, int window, int min_q, int max_q, int any_q, int tile_rows, int* status) {
+// A call as the host lays it out in one block of memory (its parts one by one cost the host 2 us more).
+struct Kv8Call {
+    void* out;                      // [n_tokens, H, D]
+    const void* q;                  // [n_tokens, H, D], tokens q_stride entries apart
+    const void *k_cache, *v_cache;  // e4m3 codes: pages page_stride bytes apart, each [page_size, KV, D]
+    const float *k_scale, *v_scale; // [num_pages, KV]
+    const int* cu_q;                // [n + 1]
+    const int* ctx_lens;            // [n]
+    const int* block_table;         // [n, table_width]
+    float* scratch;                 // of the split-key kernel: 8 * blocks * tile_rows * (D + 2) + 32 * blocks words
+    int* status;
+    cudaStream_t stream;
+    long long page_stride, q_stride;
+    int n, n_tokens, table_width, page_size, num_pages, H, KV, window;
+    int min_q, max_q;               // requests of so many new tokens are worked on
+    int any_q;                      // the most that any request may bring
+    int tile_rows;                  // split-key kernel: rows of its tiles, 8 or 16
+    int blocks;                     // split-key kernel: blocks of four warps that share the work; prompt kernel: at least as many tiles as the requests make
+    int dtype;                      // of q and out: 0 fp32, 1 bf16
+    float scale;
+};
+
+inline bool kv8_call_ok(const Kv8Call& c) {
+    return c.n >= 0 && c.n_tokens >= 0 && c.KV > 0 && c.H > 0 && c.H % c.KV == 0 && c.page_size > 0 && c.table_width >= 0 && c.num_pages >= 0 && c.window >= 0 &&
+           c.any_q >= 1 && c.min_q >= 1 && (c.dtype == 0 || c.dtype == 1);
+}
+
+inline Kv8Args kv8_args(const Kv8Call& c, int tile_rows) {
     Kv8Args a;
-    a.k_cache = (const unsigned char*)k_cache;
-    a.v_cache = (const unsigned char*)v_cache;
-    a.k_scale = k_scale;
-    a.v_scale = v_scale;
-    a.cu_q = cu_q;
-    a.ctx_lens = ctx_lens;
-    a.block_table = block_table;
-    a.n = n;
-    a.n_tokens = n_tokens;
-    a.table_width = table_width;
-    a.page_size = page_size;
-    a.num_pages = num_pages;
+    a.k_cache = (const unsigned char*)c.k_cache;
+    a.v_cache = (const unsigned char*)c.v_cache;
+    a.k_scale = c.k_scale;
+    a.v_scale = c.v_scale;
+    a.cu_q = c.cu_q;
+    a.ctx_lens = c.ctx_lens;
+    a.block_table = c.block_table;
+    a.n = c.n;
+    a.n_tokens = c.n_tokens;
+    a.table_width = c.table_width;
+    a.page_size = c.page_size;
+    a.num_pages = c.num_pages;
     a.page_shift = -1;
     for (int s = 0; s < 30; ++s)
-        if (page_size == 1 << s) a.page_shift = s;
-    a.page_stride = page_stride;
-    a.q_stride = q_stride;
-    a.H = H;
-    a.KV = KV;
-    const int group = H / KV;
+        if (c.page_size == 1 << s) a.page_shift = s;
+    a.page_stride = c.page_stride;
+    a.q_stride = c.q_stride;
+    a.H = c.H;
+    a.KV = c.KV;
+    const int group = c.H / c.KV;
     a.heads_per_tile = group < tile_rows ? group : tile_rows;
     a.tokens_per_tile = tile_rows / a.heads_per_tile;
     a.head_groups = (group + a.heads_per_tile - 1) / a.heads_per_tile;
-    a.scale = scale;
-    a.window = window;
-    a.min_q = min_q;
-    a.max_q = max_q;
-    a.any_q = any_q;
-    a.status = status;
+    a.scale = c.scale;
+    a.window = c.window;
+    a.min_q = c.min_q;
+    a.max_q = c.max_q;
+    a.any_q = c.any_q;
+    a.status = c.status;
     return a;
 }
 

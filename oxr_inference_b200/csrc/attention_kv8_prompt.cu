@@ -514,18 +514,13 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
 }  // namespace
 #endif
 
-// As oxr_kv8_attention, for bf16 queries, head sizes up to 128 and a positive scale; `tiles`: at least as many as the requests make of 256 rows.
-OXR_API int oxr_kv8_prompt_attention(void* out, const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, const int* cu_q,
-                                     const int* ctx_lens, const int* block_table, int n, int n_tokens, int table_width, int page_size, long long page_stride,
-                                     int num_pages, int H, int KV, long long q_stride, float scale, int window, int min_q, int max_q, int any_q, int tiles,
-                                     int* status, cudaStream_t stream) {
+// For bf16 queries, head sizes up to 128 and a positive scale.
+OXR_API int oxr_kv8_prompt_attention(const Kv8Call* c) {
 #if HEAD_DIM <= 128
-    if (n < 0 || n_tokens < 0 || KV <= 0 || H <= 0 || H % KV || page_size <= 0 || table_width < 0 || num_pages < 0 || window < 0 || tiles < 0) return OXR_BAD_ARGUMENT;
-    if (any_q < 2 || min_q < 1 || !(scale > 0.f)) return OXR_BAD_ARGUMENT;
-    if (tiles == 0 || n == 0 || n_tokens == 0) return 0;
-    const Kv8Args a = kv8_args(k_cache, v_cache, k_scale, v_scale, cu_q, ctx_lens, block_table, n, n_tokens, table_width, page_size, page_stride, num_pages, H,
-                               KV, q_stride, scale, window, min_q, max_q, any_q, TILE_ROWS, status);
-    const long long grid = (long long)tiles * KV * a.head_groups;
+    if (!kv8_call_ok(*c) || c->any_q < 2 || c->blocks < 0 || c->dtype != 1 || !(c->scale > 0.f)) return OXR_BAD_ARGUMENT;
+    if (c->blocks == 0 || c->n == 0 || c->n_tokens == 0) return 0;
+    const Kv8Args a = kv8_args(*c, TILE_ROWS);
+    const long long grid = (long long)c->blocks * c->KV * a.head_groups;
     if (grid > 0x7fffffffll) return OXR_BAD_ARGUMENT;
     static thread_local int ready = -1;
     int device = 0;
@@ -538,7 +533,7 @@ OXR_API int oxr_kv8_prompt_attention(void* out, const void* q, const void* k_cac
         if (cudaFuncSetAttribute(attn_kv8_prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM) != cudaSuccess) return oxr_launch_status();
         ready = device;
     }
-    oxr_launch(attn_kv8_prompt_kernel, dim3((unsigned)grid), dim3(THREADS), SMEM, stream, true, (__nv_bfloat16*)out, (const __nv_bfloat16*)q, a, tiles);
+    oxr_launch(attn_kv8_prompt_kernel, dim3((unsigned)grid), dim3(THREADS), SMEM, c->stream, true, (__nv_bfloat16*)c->out, (const __nv_bfloat16*)c->q, a, c->blocks);
     return oxr_launch_status();
 #else
     return OXR_BAD_ARGUMENT;

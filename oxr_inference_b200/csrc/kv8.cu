@@ -403,15 +403,28 @@ __global__ void __launch_bounds__(PAGE_THREADS) step_pages_kernel(const StepPage
 }
 }  // namespace
 
-// k, v [n, KV, D] (tokens k_stride / v_stride entries apart, rows 16-byte aligned) -> slots of the pools. dtype 0: fp32, 1: bf16. `ends`: scratch of
-// [num_pages][2] words, needed for more than FEW_TOKENS tokens.
-OXR_API int oxr_store_kv8(void* k_cache, void* v_cache, float* k_scale, float* v_scale, const void* k, const void* v, long long k_stride, long long v_stride,
-                          const int* slots, int n, long long page_stride, int num_pages, int page_size, int KV, int D, int dtype, int* ends, int* status,
-                          cudaStream_t stream) {
+// Calls as the host lays them out in one block of memory each.
+struct StoreCall {
+    void *k_cache, *v_cache;
+    float *k_scale, *v_scale;
+    const void *k, *v;              // [n, KV, D], tokens k_stride / v_stride entries apart, rows 16-byte aligned
+    const int* slots;
+    int* ends;                      // scratch of [num_pages][2] words, needed for more than FEW_TOKENS tokens
+    int* status;
+    cudaStream_t stream;
+    long long k_stride, v_stride, page_stride;
+    int n, num_pages, page_size, KV, D, dtype;      // dtype 0: fp32, 1: bf16
+};
+OXR_API int oxr_store_kv8(const StoreCall* c) {
+    const int n = c->n, num_pages = c->num_pages, page_size = c->page_size, KV = c->KV, D = c->D, dtype = c->dtype;
+    const long long k_stride = c->k_stride, v_stride = c->v_stride, page_stride = c->page_stride;
+    const int* slots = c->slots;
+    int *ends = c->ends, *status = c->status;
+    cudaStream_t stream = c->stream;
     if (n < 0 || num_pages < 0 || page_size <= 0 || page_size > 8192 || KV <= 0 || D <= 0 || D % 16 || (dtype != 0 && dtype != 1)) return OXR_BAD_ARGUMENT;
     if (k_stride < 0 || v_stride < 0 || k_stride > 0x7fffffffll || v_stride > 0x7fffffffll || (long long)page_size * KV * D > 0x7fffffffll) return OXR_BAD_ARGUMENT;
     if (n == 0) return 0;
-    const Kv8Pool kp = {(unsigned char*)k_cache, k_scale, k, k_stride}, vp = {(unsigned char*)v_cache, v_scale, v, v_stride};
+    const Kv8Pool kp = {(unsigned char*)c->k_cache, c->k_scale, c->k, k_stride}, vp = {(unsigned char*)c->v_cache, c->v_scale, c->v, v_stride};
     // Few tokens, most of them alone on their pages: a block per token and two KV heads, which looks through all slots itself. Many tokens: a first
     // kernel finds each page's first and last token, and a block looks after 16 tokens, a page or two.
     const bool few = n <= FEW_TOKENS;
@@ -429,14 +442,21 @@ OXR_API int oxr_store_kv8(void* k_cache, void* v_cache, float* k_scale, float* v
 }
 OXR_API int oxr_store_kv8_few() { return FEW_TOKENS; }
 
-OXR_API int oxr_step_pages(int* lengths, int* held, int* table, int* free_list, int* free_count, const int* q_lens, const int* fresh, int rows, int width,
-                           int page_size, int pool, int tokens, int* slots, int* positions, int* req_of_token, int* cu_q, int* ctx_lens, int advance, int* status,
-                           cudaStream_t stream) {
-    if (rows < 0 || rows > PAGE_ROWS || width < 0 || page_size <= 0 || pool < 0 || tokens < 0) return OXR_BAD_ARGUMENT;
+struct PagesCall {
+    int *lengths, *held, *table, *free_list, *free_count;
+    const int *q_lens, *fresh;
+    int *slots, *positions, *req_of_token, *cu_q, *ctx_lens, *status;
+    cudaStream_t stream;
+    int rows, width, page_size, pool, tokens, advance;
+};
+OXR_API int oxr_step_pages(const PagesCall* c) {
+    const int rows = c->rows, tokens = c->tokens;
+    cudaStream_t stream = c->stream;
+    if (rows < 0 || rows > PAGE_ROWS || c->width < 0 || c->page_size <= 0 || c->pool < 0 || tokens < 0) return OXR_BAD_ARGUMENT;
     // one block while its threads have a token each, else the eight of a cluster (the most that any GPU with clusters takes)
     const int blocks = tokens <= PAGE_THREADS && rows <= PAGE_THREADS ? 1 : 8;
-    const StepPages a = {lengths, held, table, free_list, free_count, q_lens, fresh, rows, width, page_size, pool, tokens,
-                         slots, positions, req_of_token, cu_q, ctx_lens, advance, blocks, status};
+    const StepPages a = {c->lengths, c->held, c->table, c->free_list, c->free_count, c->q_lens, c->fresh, rows, c->width, c->page_size, c->pool, tokens,
+                         c->slots, c->positions, c->req_of_token, c->cu_q, c->ctx_lens, c->advance, blocks, c->status};
     const size_t smem = (size_t)(5 * rows + 3) * sizeof(int);
     if (smem > 40 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(step_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (5 * PAGE_ROWS + 3) * (int)sizeof(int));

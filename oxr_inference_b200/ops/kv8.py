@@ -9,7 +9,8 @@ does on the GPU what the reference's host does between two steps (oxr_runtime/kv
 from __future__ import annotations
 
 import functools
-from ctypes import c_float, c_int, c_longlong, c_void_p
+import struct
+from ctypes import c_char_p, c_int
 from typing import NamedTuple
 
 import torch
@@ -23,6 +24,11 @@ KV8_FEW_TOKENS = 1024
 """Up to so many tokens the store looks through all slots itself; for more it takes scratch of two words a page."""
 _INT, _F32 = torch.int32, torch.float32
 
+# The calls' arguments, each in one block as the libraries declare it: pointers first, then 64-bit and 32-bit numbers.
+_ATTENTION_CALL = struct.Struct("@12Q2q14if").pack
+_STORE_CALL = struct.Struct("@10Q3q6i").pack
+_PAGES_CALL = struct.Struct("@14Q6i").pack
+
 _kv8: dict = {}
 _core = None
 
@@ -31,12 +37,11 @@ def _kv8_lib(head_dim: int):
     lib = _kv8.get(head_dim)
     if lib is None:
         lib = build.kv8_library(head_dim)
-        p, i, f, ll = c_void_p, c_int, c_float, c_longlong
-        lib.oxr_kv8_attention.argtypes = [p] * 9 + [i, i, i, i, ll, i, i, i, ll, f, i, i, i, i, i, i, p, i, p, p]
+        lib.oxr_kv8_attention.argtypes = [c_char_p]
         lib.oxr_kv8_attention.restype = c_int
-        lib.oxr_kv8_prompt_attention.argtypes = [p] * 9 + [i, i, i, i, ll, i, i, i, ll, f, i, i, i, i, i, p, p]
+        lib.oxr_kv8_prompt_attention.argtypes = [c_char_p]
         lib.oxr_kv8_prompt_attention.restype = c_int
-        lib.oxr_kv8_blocks_per_sm.argtypes = [i, i]
+        lib.oxr_kv8_blocks_per_sm.argtypes = [c_int, c_int]
         lib.oxr_kv8_blocks_per_sm.restype = c_int
         lib.oxr_kv8_head_dim.restype = c_int
         if lib.oxr_kv8_head_dim() != head_dim:
@@ -52,11 +57,11 @@ def _core_lib():
     global _core
     if _core is None:
         lib = ops._lib()
-        p, i, ll = c_void_p, c_int, c_longlong
-        lib.oxr_store_kv8.argtypes = [p, p, p, p, p, p, ll, ll, p, i, ll, i, i, i, i, i, p, p, p]
+        lib.oxr_store_kv8.argtypes = [c_char_p]
         lib.oxr_store_kv8.restype = c_int
-        lib.oxr_step_pages.argtypes = [p] * 7 + [i] * 5 + [p] * 5 + [i, p, p]
+        lib.oxr_step_pages.argtypes = [c_char_p]
         lib.oxr_step_pages.restype = c_int
+        lib.oxr_store_kv8_few.restype = c_int
         if lib.oxr_store_kv8_few() != KV8_FEW_TOKENS:
             raise BuildError(f"the store's kernels take up to {lib.oxr_store_kv8_few()} tokens without scratch, the host {KV8_FEW_TOKENS}")
         _core = lib
@@ -147,8 +152,9 @@ def store_kv8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: to
     if n == 0:
         return
     ends = None if n <= KV8_FEW_TOKENS else slots.new_empty(2 * pages)
-    ops._done(_core_lib().oxr_store_kv8(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k.data_ptr(), v.data_ptr(), k_stride,
-                                        v_stride, slots.data_ptr(), n, page_stride, pages, page, kv, d, code, ops._ptr(ends), status.data_ptr(), ops._stream()), "store_kv8")
+    call = _STORE_CALL(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k.data_ptr(), v.data_ptr(), slots.data_ptr(),
+                       0 if ends is None else ends.data_ptr(), status.data_ptr(), ops._stream(), k_stride, v_stride, page_stride, n, pages, page, kv, d, code)
+    ops._done(_core_lib().oxr_store_kv8(call), "store_kv8")
     if ends is not None:
         ops.launch_count += 1
 
@@ -227,14 +233,17 @@ def paged_attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         return out
     lib = _kv8_lib(d)
     group = heads // kv
-    common = (out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), cu_q.data_ptr(), ctx_lens.data_ptr(),
-              block_table.data_ptr(), n, tokens, block_table.shape[1], page, page_stride, pages, heads, kv, q_stride, float(scale), int(window))
+    stream = ops._stream()
+    pointers = (out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), cu_q.data_ptr(), ctx_lens.data_ptr(),
+                block_table.data_ptr())
+    sizes = (page_stride, q_stride, n, tokens, block_table.shape[1], page, pages, heads, kv, int(window))
     longest = max_q_len = int(max_q_len)
     seen = max(1, min(kv_len_bound, window + max_q_len) if window > 0 else kv_len_bound)
     if kv8_prompt_takes(max_q_len, d, q.dtype, scale) and kv8_prompt_pays(n, tokens, max_q_len, heads, kv, d, seen):
         fewest = ops.SHORT_MAX_TOKENS + 1 if n > 1 else 1      # a request alone goes there whatever it brings
         tiles = min(tokens, min(n, tokens // fewest) + tokens // (KV8_PROMPT_ROWS // min(group, KV8_PROMPT_ROWS)))
-        ops._done(lib.oxr_kv8_prompt_attention(*common, fewest, max_q_len, max_q_len, tiles, status.data_ptr(), ops._stream()), "paged_attention_kv8 (prompts)")
+        call = _ATTENTION_CALL(*pointers, 0, status.data_ptr(), stream, *sizes, fewest, max_q_len, max_q_len, 0, tiles, code, scale)
+        ops._done(lib.oxr_kv8_prompt_attention(call), "paged_attention_kv8 (prompts)")
         longest = fewest - 1
         if longest == 0:
             return out
@@ -245,7 +254,8 @@ def paged_attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     seen = min(kv_len_bound, window + longest + 32) if window > 0 else kv_len_bound
     blocks = kv8_blocks(tiles, max(1, -(-seen // 32)), _kv8_room(d, code, rows))
     scratch = k_scale.new_empty(8 * blocks * rows * (d + 2) + 32 * blocks)
-    ops._done(lib.oxr_kv8_attention(*common, 1, longest, max_q_len, rows, blocks, scratch.data_ptr(), code, status.data_ptr(), ops._stream()), "paged_attention_kv8")
+    call = _ATTENTION_CALL(*pointers, scratch.data_ptr(), status.data_ptr(), stream, *sizes, 1, longest, max_q_len, rows, blocks, code, scale)
+    ops._done(lib.oxr_kv8_attention(call), "paged_attention_kv8")
     ops.launch_count += 1
     return out
 
@@ -299,8 +309,8 @@ def step_pages(lengths: torch.Tensor, held: torch.Tensor, block_table: torch.Ten
     block = block_table.new_empty(3 * tokens + 2 * rows + 1)
     step = PageStep(*torch.split_with_sizes(block, (tokens, tokens, tokens, rows + 1, rows)))
     at = block.data_ptr()
-    ops._done(_core_lib().oxr_step_pages(lengths.data_ptr(), held.data_ptr(), block_table.data_ptr(), free_list.data_ptr(), free_count.data_ptr(),
-                                         q_lens.data_ptr(), ops._ptr(fresh), rows, width, int(page_size), free_list.shape[0], int(tokens), at,
-                                         at + 4 * tokens, at + 8 * tokens, at + 12 * tokens, at + 4 * (3 * tokens + rows + 1), int(advance),
-                                         status.data_ptr(), ops._stream()), "step_pages")
+    call = _PAGES_CALL(lengths.data_ptr(), held.data_ptr(), block_table.data_ptr(), free_list.data_ptr(), free_count.data_ptr(), q_lens.data_ptr(),
+                       0 if fresh is None else fresh.data_ptr(), at, at + 4 * tokens, at + 8 * tokens, at + 12 * tokens, at + 4 * (3 * tokens + rows + 1),
+                       status.data_ptr(), ops._stream(), rows, width, page_size, free_list.shape[0], tokens, 1 if advance else 0)
+    ops._done(_core_lib().oxr_step_pages(call), "step_pages")
     return step
