@@ -440,7 +440,9 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
         cp_async_wait<STAGES - 2>();
         const int slot = (turn + i) % STAGES;
         if (TMA && !mbar_wait(bars + slot, ((turn + i) / STAGES) & 1)) {
-            if (lane == 0) oxr_report(a.status, OXR_WAIT_EXPIRED, 40);
+            // what is on its way has to arrive before the block's memory is another's; nothing of this stretch is to be joined
+            if (lane == 0) { oxr_report(a.status, OXR_WAIT_EXPIRED, 40); left.cuts[me].last = -1; }
+            for (int k = i + 1; k < min(i + STAGES, mine); ++k) mbar_wait(bars + (turn + k) % STAGES, ((turn + k) / STAGES) & 1);
             cp_async_wait<0>();
             return;
         }

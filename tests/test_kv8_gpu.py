@@ -332,6 +332,12 @@ def test_attention_bad_pages_and_lengths_are_reported(status):
         status.zero_()
 
 
+def test_attention_bounds_beyond_all_sizes(status):
+    """A window, a number of new tokens and a length that no 32-bit number holds mean none at all. (They decide how the keys are cut, and with it the order
+    of the sums.)"""
+    Batch([1, 4, 2], [60, 35, 90], heads=4, kv=2, d=64, page=16, dtype=torch.bfloat16).check(status, window=1 << 40, max_q_len=1 << 40, kv_len_bound=1 << 40)
+
+
 def test_attention_far_pages(status):
     """Pages beyond 2^31 bytes of the pool."""
     d, kv, page = 128, 8, 64

@@ -52,6 +52,7 @@ def bad_pools():
         "pages apart differently": (torch.zeros((3, 2, 16, 2, 32)).to(E4M3)[:, 0], v, ks, vs), "head size": (*pools(d=24)[:2], ks, vs),
         "not aligned": (odd if odd.data_ptr() % 16 else odd.flatten()[8:], v, ks, vs), "scales of another type": (k, v, ks.double(), vs),
         "scales of other sizes": (k, v, ks, vs[:2]), "scales with strides": (k, v, ks, torch.zeros((3, 4))[:, ::2]), "three dimensions": (k[0], v[0], ks, vs),
+        "no pages": pools(pages=0), "no places": pools(page=0),
     }
 
 
@@ -94,6 +95,12 @@ def test_bad_attention_calls(on_cpu):
                    dict(out=torch.zeros((3, 4, 32)).bfloat16()), dict(out=torch.zeros((3, 4, 64))[..., :32])):
         with pytest.raises(ops.KernelError):
             call(**change)
+    both = torch.zeros((5, 4, 32))
+    for q, out in ((both[:3], both[:3]), (both[1:4], both[2:5]), (torch.zeros((3, 6, 32))[:, :4], None)):
+        if out is None:      # columns of a wider product; its memory as output
+            out = torch.as_strided(q, (3, 4, 32), (128, 32, 1))
+        with pytest.raises(ops.KernelError, match="over q"):
+            call(q=q, out=out)
     # nothing to do: no library is needed
     assert call(q=torch.zeros((0, 4, 32))).shape == (0, 4, 32)
     out = torch.full((3, 4, 32), 5.0)
@@ -106,7 +113,7 @@ def test_bad_tables(on_cpu):
                 fresh=None, page_size=16, tokens=5, status=status())
     for change in (dict(lengths=row[:2]), dict(held=row.long()), dict(q_lens=torch.zeros(4, dtype=INT)), dict(fresh=row[:1]), dict(fresh=row.bool()), dict(page_size=0),
                    dict(tokens=-1), dict(free_count=row), dict(free_list=torch.zeros((3, 3), dtype=INT)), dict(block_table=row),
-                   dict(block_table=torch.zeros((3, 8), dtype=INT)[:, ::2])):
+                   dict(block_table=torch.zeros((3, 8), dtype=INT)[:, ::2]), dict(page_size=1 << 29), dict(page_size=1 << 28), dict(tokens=1 << 30)):
         with pytest.raises(ops.KernelError):
             ops.step_pages(**{**good, **change})
     many = torch.zeros(8193, dtype=INT)
