@@ -8,7 +8,7 @@ from typing import Any, Mapping
 import torch
 
 from oxr_inference_b200 import ops
-from oxr_inference_b200.cache.manager import CacheManager
+from oxr_inference_b200.cache.manager import CacheManager, RequestCache
 from oxr_inference_b200.config.model_config import read_config_json
 from oxr_inference_b200.config.registry import resolve_architecture
 from oxr_inference_b200.engine.batch import BatchBuilder, StepEntry
@@ -46,6 +46,7 @@ class ModelRunner:
                                   device=rt.device, dtype=rt.dtype)
         self.builder = BatchBuilder(self.cache, model.tile_specs, rt.device, rt.status)
         self.steps = 0
+        self._device_decode = None
 
     # ---- construction
     @staticmethod
@@ -102,6 +103,15 @@ class ModelRunner:
                 self.cache.advance(e.cache, e.cache.length + len(e.tokens))
         self.steps += 1
         return logits
+
+    def decode(self, requests: list[RequestCache], tokens: list[int], steps: int) -> list[list[int]]:
+        """The next ``steps`` tokens of each request, chosen greedily on the GPU with no host work between the steps (see :class:`DeviceDecode`);
+        ``tokens``: the last token of each, not yet in its cache."""
+        from oxr_inference_b200.engine.device_decode import DeviceDecode
+
+        if self._device_decode is None:
+            self._device_decode = DeviceDecode(self)
+        return self._device_decode.run(requests, tokens, steps)
 
     def check(self) -> None:
         """Raise if any kernel reported an error since the last check (synchronises)."""
