@@ -140,7 +140,7 @@ def store_kv8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: to
     A page's scale is a power of two, one for each KV head and for keys and values apart: the least 2^e whose 448-fold reaches every magnitude stored since
     the page was begun. Storing a page's first slot begins it (what its other slots held is void); after that the scale only grows, and what the
     page holds is then rounded to the new scale (exact but for codes below e4m3's normal range). Infinities and NaN become NaN and have no say in
-    the scale. A slot outside the pool sets the status word and is skipped. Measured on a B200 (8 KV heads of 128): 64 tokens 2.9 us, 8,192 tokens 11 us."""
+    the scale. A slot outside the pool sets the status word and is skipped. Measured on a B200 (8 KV heads of 128): 64 tokens 3.3 us, 10,300 tokens 23 us."""
     _here(k_cache, "k_cache")
     device = k_cache.get_device()
     pages, page, kv, d, page_stride = _need_pools(device, k_cache, v_cache, k_scale, v_scale)
