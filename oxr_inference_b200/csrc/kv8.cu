@@ -94,9 +94,10 @@ __global__ void store_kv8_ends_kernel(int* __restrict__ ends, const int* __restr
 constexpr int FEW_TOKENS = 1024;
 constexpr int HELD = 8;   // groups of eight entries that a lane keeps between the two looks at them: pages of up to 2,048 entries a head
 
-// EIGHTS: D / 8 where that divides a warp, else 0 (taken from D).
+// EIGHTS: D / 8 where that divides a warp, else 0 (taken from D). Blocks an SM: the held groups want 80 registers of 16-bit entries; at 72 (seven blocks)
+// 10,300 tokens of 8 heads of 128 take 22 us, at 80 (six) 23.3.
 template <typename T, int EIGHTS>
-__global__ void __launch_bounds__(128, sizeof(T) == 4 ? 4 : 6) store_kv8_kernel(const Kv8Pool kp, const Kv8Pool vp, const int* __restrict__ slots, const int* __restrict__ ends, int n,
+__global__ void __launch_bounds__(128, sizeof(T) == 4 ? 4 : 7) store_kv8_kernel(const Kv8Pool kp, const Kv8Pool vp, const int* __restrict__ slots, const int* __restrict__ ends, int n,
                                                            long long page_stride, int num_pages, int page_size, int KV, int D, int tokens_per_block, int* status) {
     extern __shared__ int winner[];   // [page_size] the token that is stored at each place of the page, or -1
     pdl_wait();

@@ -85,7 +85,7 @@ def _here(t: torch.Tensor, name: str) -> None:
 
 
 # The checks are laid out for calls that pass them: a few comparisons in one expression each, and a function that finds the words for one that does not.
-# (Outside of CUDA graphs a small step's calls are bound by the host: attention 19 us a call instead of 23, tables 14 instead of 19, the store 9.5 instead of 11.5.)
+# (Outside of CUDA graphs a small step's calls are bound by the host: attention 17.7 us a call instead of 23, tables 14 instead of 19, the store 9.2 instead of 11.5.)
 def _plain(t: torch.Tensor, device: int, dtype: torch.dtype) -> bool:
     return t.dtype is dtype and t.is_contiguous() and t.get_device() == device
 
@@ -106,15 +106,16 @@ def _need_pools(device: int, k_cache: torch.Tensor, v_cache: torch.Tensor, k_sca
     if not (pages and page and kv and d):
         raise ops.KernelError(f"pools of {tuple(shape)}: there is nothing in them")
     row = kv * d
-    if (strides[1:] != (row, d, 1) or v_cache.stride() != strides or strides[0] < page * row or strides[0] % 16 or d % 16
-            or (k_cache.data_ptr() | v_cache.data_ptr()) % 16 or k_cache.get_device() != device or v_cache.get_device() != device):
+    stride = strides[0]
+    if (strides != (stride, row, d, 1) or v_cache.stride() != strides or stride < page * row or (stride | d | k_cache.data_ptr() | v_cache.data_ptr()) % 16
+            or k_cache.get_device() != device or v_cache.get_device() != device):
         raise ops.KernelError(f"pools with strides {strides} and {v_cache.stride()}: pages must be whole, 16-byte aligned and as far apart in both, "
                               f"head sizes multiples of 16, on cuda:{device}")
-    if not (_plain(k_scale, device, _F32) and _plain(v_scale, device, _F32)):
+    if not (k_scale.dtype is v_scale.dtype is _F32 and k_scale.is_contiguous() and v_scale.is_contiguous() and k_scale.get_device() == v_scale.get_device() == device):
         _refuse_plain(device, _F32, k_scale=k_scale, v_scale=v_scale)
     if k_scale.shape != (pages, kv) or v_scale.shape != (pages, kv):
         raise ops.KernelError(f"one scale per page and KV head: {tuple(k_scale.shape)}, {tuple(v_scale.shape)} for pools of {pages} pages and {kv} heads")
-    return pages, page, kv, d, strides[0]
+    return pages, page, kv, d, stride
 
 
 def _head_rows(t: torch.Tensor, name: str, device: int) -> int:
@@ -140,7 +141,7 @@ def store_kv8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: to
     A page's scale is a power of two, one for each KV head and for keys and values apart: the least 2^e whose 448-fold reaches every magnitude stored since
     the page was begun. Storing a page's first slot begins it (what its other slots held is void); after that the scale only grows, and what the
     page holds is then rounded to the new scale (exact but for codes below e4m3's normal range). Infinities and NaN become NaN and have no say in
-    the scale. A slot outside the pool sets the status word and is skipped. Measured on a B200 (8 KV heads of 128): 64 tokens 3.3 us, 10,300 tokens 23 us."""
+    the scale. A slot outside the pool sets the status word and is skipped. Measured on a B200 (8 KV heads of 128): 64 tokens 3.3 us, 10,300 tokens 22 us."""
     _here(k_cache, "k_cache")
     device = k_cache.get_device()
     pages, page, kv, d, page_stride = _need_pools(device, k_cache, v_cache, k_scale, v_scale)
@@ -161,6 +162,18 @@ def store_kv8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: to
     ops._done(_core_lib().oxr_store_kv8(call), "store_kv8")
     if ends is not None:
         ops.launch_count += 1
+
+
+@functools.lru_cache(maxsize=4096)
+def _split_plan(requests: int, tokens: int, longest: int, group: int, kv: int, head_dim: int, code: int, seen: int) -> tuple[int, int, int]:
+    """(rows of a tile, blocks, words of scratch) of the split-key kernel for portions of up to ``longest`` tokens; a tile's rows are (token, query head) pairs of
+    one KV head."""
+    rows = 8 if group * longest <= 8 else 16
+    heads_per_tile = min(group, rows)
+    per_tile = rows // heads_per_tile
+    tiles = min(tokens, requests * -(-longest // per_tile), requests + tokens // per_tile) * kv * -(-group // heads_per_tile)
+    blocks = kv8_blocks(tiles, -(-seen // 32), _kv8_room(head_dim, code, rows))
+    return rows, blocks, 8 * blocks * rows * (head_dim + 2) + 32 * blocks
 
 
 @functools.lru_cache(maxsize=None)
@@ -228,7 +241,9 @@ def paged_attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         raise ops.KernelError(f"q {tuple(q.shape)} does not fit {kv} KV heads of {d}")
     tokens, heads = q.shape[0], q.shape[1]
     q_stride = _head_rows(q, "q", device)
-    if not (_plain(cu_q, device, _INT) and _plain(ctx_lens, device, _INT) and _plain(block_table, device, _INT) and _plain(status, device, _INT)):
+    if not (cu_q.dtype is ctx_lens.dtype is block_table.dtype is status.dtype is _INT and cu_q.is_contiguous() and ctx_lens.is_contiguous()
+            and block_table.is_contiguous() and status.is_contiguous()
+            and cu_q.get_device() == ctx_lens.get_device() == block_table.get_device() == status.get_device() == device):
         _refuse_plain(device, _INT, cu_q=cu_q, ctx_lens=ctx_lens, block_table=block_table, status=status)
     n = ctx_lens.shape[0]
     if ctx_lens.dim() != 1 or cu_q.shape != (n + 1,) or block_table.dim() != 2 or block_table.shape[0] != n:
@@ -252,7 +267,7 @@ def paged_attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
                 block_table.data_ptr())
     sizes = (page_stride, q_stride, n, tokens, block_table.shape[1], page, pages, heads, kv, window)
     seen = max(1, min(kv_len_bound, window + max_q_len) if window > 0 else kv_len_bound)
-    if kv8_prompt_takes(max_q_len, d, q.dtype, scale) and kv8_prompt_pays(n, tokens, max_q_len, heads, kv, d, seen):
+    if max_q_len > ops.SHORT_MAX_TOKENS and kv8_prompt_takes(max_q_len, d, q.dtype, scale) and kv8_prompt_pays(n, tokens, max_q_len, heads, kv, d, seen):
         fewest = ops.SHORT_MAX_TOKENS + 1 if n > 1 else 1      # a request alone goes there whatever it brings
         tiles = min(tokens, min(n, tokens // fewest) + tokens // (KV8_PROMPT_ROWS // min(group, KV8_PROMPT_ROWS)))
         call = _ATTENTION_CALL(*pointers, 0, status.data_ptr(), stream, *sizes, fewest, max_q_len, max_q_len, 0, tiles, code, scale)
@@ -260,13 +275,9 @@ def paged_attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         longest = fewest - 1
         if longest == 0:
             return out
-    rows = 8 if group * longest <= 8 else 16      # the split-key kernel's tiles: (token, query head) pairs of one KV head
-    heads_per_tile = min(group, rows)
-    per_tile = rows // heads_per_tile
-    tiles = min(tokens, n * -(-longest // per_tile), n + tokens // per_tile) * kv * -(-group // heads_per_tile)
-    seen = min(kv_len_bound, window + longest + 32) if window > 0 else kv_len_bound
-    blocks = kv8_blocks(tiles, max(1, -(-seen // 32)), _kv8_room(d, code, rows))
-    scratch = k_scale.new_empty(8 * blocks * rows * (d + 2) + 32 * blocks)
+    seen = max(1, min(kv_len_bound, window + longest + 32) if window > 0 else kv_len_bound)
+    rows, blocks, words = _split_plan(n, tokens, longest, group, kv, d, code, seen)
+    scratch = k_scale.new_empty(words)
     call = _ATTENTION_CALL(*pointers, scratch.data_ptr(), status.data_ptr(), stream, *sizes, 1, longest, max_q_len, rows, blocks, code, scale)
     ops._done(lib.oxr_kv8_attention(call), "paged_attention_kv8")
     ops.launch_count += 1
@@ -303,8 +314,10 @@ def step_pages(lengths: torch.Tensor, held: torch.Tensor, block_table: torch.Ten
     ``tokens`` tokens, the status word is set, nothing moves, and the arrays hold no token at all (slots -1, ``cu_q`` and ``ctx_lens`` 0)."""
     _here(block_table, "block_table")
     device = block_table.get_device()
-    if not (_plain(lengths, device, _INT) and _plain(held, device, _INT) and _plain(block_table, device, _INT) and _plain(free_list, device, _INT)
-            and _plain(free_count, device, _INT) and _plain(q_lens, device, _INT) and _plain(status, device, _INT)):
+    if not (lengths.dtype is held.dtype is block_table.dtype is free_list.dtype is free_count.dtype is q_lens.dtype is status.dtype is _INT
+            and lengths.is_contiguous() and held.is_contiguous() and block_table.is_contiguous() and free_list.is_contiguous() and free_count.is_contiguous()
+            and q_lens.is_contiguous() and status.is_contiguous()
+            and lengths.get_device() == held.get_device() == free_list.get_device() == free_count.get_device() == q_lens.get_device() == status.get_device() == device):
         _refuse_plain(device, _INT, lengths=lengths, held=held, block_table=block_table, free_list=free_list, free_count=free_count, q_lens=q_lens, status=status)
     if block_table.dim() != 2:
         raise ops.KernelError(f"block_table must be [rows, pages], got {tuple(block_table.shape)}")
