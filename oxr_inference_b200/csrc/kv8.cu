@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 4 : 7) store_kv8_kernel(
     for (unsigned runs = __ballot_sync(0xffffffffu, begins); runs; runs &= runs - 1) {     // the same in every warp
         const int i = i0 + __ffs(runs) - 1;
         const int page = __ldg(slots + i) / page_size, first = page * page_size;   // below 2^31, as the slot is
-        auto here = [&](int s) { return (unsigned)(s - first) < (unsigned)page_size; };   // (negative slots wrap far above)
+        auto here = [&](int s) { return (unsigned)s - (unsigned)first < (unsigned)page_size; };   // (negative slots wrap above it: `first` is 8,192 and more below 2^31)
         const int u = 2 * blockIdx.y * 2 + warp, h = u >> 1;      // this warp's head and whether it has the keys or the values
         const Kv8Pool& pool = (u & 1) ? vp : kp;
         const unsigned x_stride = (unsigned)pool.x_stride;
@@ -397,7 +397,8 @@ __global__ void __launch_bounds__(PAGE_THREADS) step_pages_kernel(const StepPage
         }
         const int pos = begin[low] + t - cu[low], j = pos / a.page_size, k = keeps[low];
         const int page = j < k ? a.table[(size_t)low * a.width + j] : a.free_list[top - 1 - (taken[low] + j - k)];
-        a.slots[t] = page < 0 ? -1 : page * a.page_size + pos % a.page_size;
+        const long long slot = (long long)page * a.page_size + pos % a.page_size;
+        a.slots[t] = page < 0 ? -1 : (int)min(slot, 0x7fffffffll);      // a number that no page has stays one that no pool has, and the store reports it
         a.positions[t] = pos;
         a.req_of_token[t] = low;
     }
@@ -423,7 +424,8 @@ OXR_API int oxr_store_kv8(const StoreCall* c) {
     int *ends = c->ends, *status = c->status;
     cudaStream_t stream = c->stream;
     if (n < 0 || num_pages < 0 || page_size <= 0 || page_size > 8192 || KV <= 0 || D <= 0 || D % 16 || (dtype != 0 && dtype != 1)) return OXR_BAD_ARGUMENT;
-    if (k_stride < 0 || v_stride < 0 || k_stride > 0x7fffffffll || v_stride > 0x7fffffffll || (long long)page_size * KV * D > 0x7fffffffll) return OXR_BAD_ARGUMENT;
+    if (k_stride < 0 || v_stride < 0 || k_stride > 0x7fffffffll || v_stride > 0x7fffffffll || (long long)page_size * KV * D > 0x7fffffffll
+        || (long long)num_pages * page_size > 0x80000000ll - 8192) return OXR_BAD_ARGUMENT;
     if (n == 0) return 0;
     const Kv8Pool kp = {(unsigned char*)c->k_cache, c->k_scale, c->k, k_stride}, vp = {(unsigned char*)c->v_cache, c->v_scale, c->v, v_stride};
     // Few tokens, most of them alone on their pages: a block per token and two KV heads, which looks through all slots itself. Many tokens: a first

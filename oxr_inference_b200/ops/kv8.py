@@ -151,8 +151,8 @@ def store_kv8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: to
     if slots.dim() != 1 or k.shape != (n, kv, d) or v.shape != (n, kv, d) or k.dtype != v.dtype:
         raise ops.KernelError(f"k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} must be [{n}, {kv}, {d}] of one dtype for {n} slots")
     code = ops._dtype_code(k)
-    if page > 8192:
-        raise ops.KernelError(f"pages of {page} tokens: the store takes up to 8192")
+    if page > 8192 or pages * page > 0x80000000 - 8192:
+        raise ops.KernelError(f"{pages} pages of {page} tokens: the store takes pages of up to 8192, slots below 2^31 - 8192")
     k_stride, v_stride = _head_rows(k, "k", device), _head_rows(v, "v", device)
     if n == 0:
         return
@@ -311,7 +311,8 @@ def step_pages(lengths: torch.Tensor, held: torch.Tensor, block_table: torch.Ten
     as cached), without it the same step may be asked for again and takes nothing more.
 
     All or nothing: if pages are lacking, a row does not fit its numbers (longer than ``width`` pages, a negative length) or the step brings more than
-    ``tokens`` tokens, the status word is set, nothing moves, and the arrays hold no token at all (slots -1, ``cu_q`` and ``ctx_lens`` 0)."""
+    ``tokens`` tokens, the status word is set, nothing moves, and the arrays hold no token at all (slots -1, ``cu_q`` and ``ctx_lens`` 0). The numbers of
+    pages are taken as they stand: a token on a negative one gets slot -1, on one beyond all pools a slot that the store reports."""
     _here(block_table, "block_table")
     device = block_table.get_device()
     if not (lengths.dtype is held.dtype is block_table.dtype is free_list.dtype is free_count.dtype is q_lens.dtype is status.dtype is _INT

@@ -521,3 +521,12 @@ def test_a_prompt_and_its_decoding_in_a_graph(status, dtype):
         graph.replay()
         check(s, o, q, k, v, [1] * rows)
     assert lengths.tolist() == [p + steps for p in prompts]
+
+
+def test_tables_of_page_numbers_beyond_all_pools(status):
+    """They do not come round to the pages below: 2^29 pages of 8 are as many slots as 32 bits count."""
+    far = [1 << 28, 1 << 29, (1 << 29) + 3, (1 << 31) - 1, -2, 5]
+    case = ([8] * 6, [2] * 6, [[0, f] for f in far], ([1, 2, 3], 3), [1] * 6, [0] * 6)
+    state, step = run_tables(case, 8, 6, status)
+    fine(status)
+    assert step.slots.tolist() == [(1 << 31) - 1] * 4 + [-1, 40]

@@ -152,3 +152,13 @@ def test_plain_pages_give_back_and_take():
     held, table, stack, count, begin, cu = P.pages([20, 5], [2, 1], [[7, 8, -1], [9, -1, -1]], ([3, 4, -1, -1, -1], 2), [1, 30], [1, 0], 16)
     assert (held, begin, cu, count) == ([1, 3], [0, 5], [0, 1, 31], 1)
     assert table[0][0] == 8 and table[1] == [9, 7, 4] and stack[:1] == [3]
+
+
+def test_pools_of_more_slots_than_there_are_numbers(on_cpu):
+    pages = (1 << 27) - 511      # of 16 tokens: 2^31 - 8176 slots
+    k, v, scales = torch.empty((pages, 16, 1, 16), dtype=E4M3, device="meta"), torch.empty((pages, 16, 1, 16), dtype=E4M3, device="meta"), torch.empty((pages, 1), device="meta")
+    x, slots = (torch.empty((1, 1, 16), device="meta"), torch.empty(1, dtype=INT, device="meta"))
+    with pytest.raises(ops.KernelError, match="slots below"):
+        ops.store_kv8(x, x, slots, k, v, scales, scales, torch.empty(4, dtype=INT, device="meta"))
+    # one page less: with no tokens there is nothing left to do
+    ops.store_kv8(x[:0], x[:0], slots[:0], k[1:], v[1:], scales[1:], scales[1:], torch.empty(4, dtype=INT, device="meta"))
