@@ -347,7 +347,7 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
                                     kvh * D + pnl * PW, a.in_page(key0 + pc * piece), from, bar);
                 }
             } else {
-                const long long row = good ? (long long)page * a.page_stride + (a.in_page(key) * a.KV + kvh) * D : -1;
+                const long long row = good ? (long long)page * a.page_stride + a.row_in_page(key, kvh) : -1;
 #pragma unroll
                 for (int c = 0; c < KSTEPS; ++c) {
                     const int chunk = c * 32 + lane, r = chunk / KSTEPS, col = chunk % KSTEPS;
@@ -359,7 +359,7 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
                     cp_async16(dst + TENSOR_BYTES, a.v_cache + off, take);
                 }
             }
-            const int sc = good ? page * a.KV + kvh : 0;
+            const size_t sc = good ? (size_t)page * a.KV + kvh : 0;      // pools of small pages have more scales than 32 bits count
             const uint32_t scale_at = my_scales + slot * SCALE_BYTES + lane * 4;
             cp_async4(scale_at, a.k_scale + sc, good);
             cp_async4(scale_at + KEYS * 4, a.v_scale + sc, good);

@@ -33,6 +33,8 @@ struct Kv8Args {
 
     __device__ __forceinline__ int page_of(int key) const { return page_shift >= 0 ? key >> page_shift : key / page_size; }
     __device__ __forceinline__ int in_page(int key) const { return page_shift >= 0 ? key & (page_size - 1) : key % page_size; }
+    // bytes from the start of its page to a key's row of a KV head (a page may be of more than 2^31)
+    __device__ __forceinline__ long long row_in_page(int key, int kvh) const { return ((long long)in_page(key) * KV + kvh) * D; }
 };
 
 // A call as the host lays it out in one block of memory (its parts one by one cost the host 2 us more).
@@ -58,7 +60,7 @@ struct Kv8Call {
 };
 
 inline bool kv8_call_ok(const Kv8Call& c) {
-    return c.n >= 0 && c.n_tokens >= 0 && c.KV > 0 && c.H > 0 && c.H % c.KV == 0 && c.page_size > 0 && c.table_width >= 0 && c.num_pages >= 0 && c.window >= 0 &&
+    return c.n >= 0 && c.n_tokens >= 0 && c.KV > 0 && (long long)c.KV * D <= 0x7fffffffll && c.H > 0 && c.H % c.KV == 0 && c.page_size > 0 && c.table_width >= 0 && c.num_pages >= 0 && c.window >= 0 &&
            c.any_q >= 1 && c.min_q >= 1 && (c.dtype == 0 || c.dtype == 1);
 }
 

@@ -206,7 +206,7 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                 if (lt >= KEYS) return;
                 BlockInfo& f = sh.info[b % INFO];
                 const int key = (block0 + b) * KEYS + lt;
-                f.row[lt] = page >= 0 ? (long long)page * a.page_stride + (a.in_page(key) * a.KV + kvh) * D : -1;
+                f.row[lt] = page >= 0 ? (long long)page * a.page_stride + a.row_in_page(key, kvh) : -1;
                 f.k_scale[lt] = ks;
                 f.v_scale[lt] = vs;
                 // (positive floats compare as integers do)
@@ -499,7 +499,7 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                         const int page = __ldg(table_row + a.page_of(key));
                         if (page < 0 || page >= a.num_pages) continue;
                         const bool finite = fabsf(__ldg(a.v_scale + (size_t)page * a.KV + kvh)) < INFINITY;
-                        const unsigned char* codes = a.v_cache + (long long)page * a.page_stride + (a.in_page(key) * a.KV + kvh) * D;
+                        const unsigned char* codes = a.v_cache + (long long)page * a.page_stride + a.row_in_page(key, kvh);
                         for (int d = 0; d < D; ++d)
                             if (!finite || (__ldg(codes + d) & 0x7f) == 0x7f) dst[d] = __float2bfloat16_rn(__uint_as_float(0x7fffffffu));
                     }

@@ -87,8 +87,8 @@ __global__ void store_kv8_ends_kernel(int* __restrict__ ends, const int* __restr
     const int s = i < n ? __ldg(slots + i) : -1;
     if (s < 0 || s / page_size >= num_pages) return;
     const int page = s / page_size, before = i > 0 ? __ldg(slots + i - 1) : -1, after = i + 1 < n ? __ldg(slots + i + 1) : -1;
-    if (before < 0 || before / page_size != page) atomicMin(reinterpret_cast<unsigned*>(ends) + 2 * page, (unsigned)i);
-    if (after < 0 || after / page_size != page) atomicMax(ends + 2 * page + 1, i);
+    if (before < 0 || before / page_size != page) atomicMin(reinterpret_cast<unsigned*>(ends) + 2ll * page, (unsigned)i);
+    if (after < 0 || after / page_size != page) atomicMax(ends + 2ll * page + 1, i);
 }
 
 constexpr int FEW_TOKENS = 1024;
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 4 : 7) store_kv8_kernel(
             if (page >= num_pages) {
                 if (warp == 0 && blockIdx.y == 0) oxr_report(status, OXR_BAD_SLOT, i0 + lane);
             } else {
-                begins = (before < 0 || before / page_size != page) && (ends == nullptr || __ldg(ends + 2 * page) == i0 + lane);
+                begins = (before < 0 || before / page_size != page) && (ends == nullptr || __ldg(ends + 2ll * page) == i0 + lane);
             }
         }
     }
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 4 : 7) store_kv8_kernel(
         const unsigned x_stride = (unsigned)pool.x_stride;
         float* where = pool.scale + (size_t)page * KV + h;
         const float before = h < KV ? *where : 0.f;
-        const int last = ends != nullptr ? __ldg(ends + 2 * page + 1) : n - 1;
+        const int last = ends != nullptr ? __ldg(ends + 2ll * page + 1) : n - 1;
         for (int j = threadIdx.x; j < page_size; j += blockDim.x) winner[j] = -1;
         if (ends == nullptr) {
             bool earlier = false;

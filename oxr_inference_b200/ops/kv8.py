@@ -106,6 +106,8 @@ def _need_pools(device: int, k_cache: torch.Tensor, v_cache: torch.Tensor, k_sca
     if not (pages and page and kv and d):
         raise ops.KernelError(f"pools of {tuple(shape)}: there is nothing in them")
     row = kv * d
+    if max(pages, page, row) > 0x7fffffff:
+        raise ops.KernelError(f"pools of {tuple(shape)}: pages, their tokens and the bytes of a token are counted in 32 bits")
     stride = strides[0]
     if (strides != (stride, row, d, 1) or v_cache.stride() != strides or stride < page * row or (stride | d | k_cache.data_ptr() | v_cache.data_ptr()) % 16
             or k_cache.get_device() != device or v_cache.get_device() != device):
