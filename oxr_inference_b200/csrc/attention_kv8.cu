@@ -15,9 +15,14 @@
 // lost); an fp32 query is the sum of two fp16 numbers to 22 bits. The weights are rounded to fp16 (11 bits) against the row's running maximum, times
 // 2^15 so that they keep their bits down to 2^-29 of it; with fp32 queries they are two numbers as well.
 //
-// The weights of a block of keys are taken against the maximum of s_j + log2(vs) instead of s_j: weights times scales then never exceed one
-// however much the scales of pages differ, and a rescaled sum needs nothing but the usual factor. (log2(vs) stands for the integer 2^lv >= the
-// block's largest scale, relative to the scale of the last page, so that neither sums nor weights leave the fp32 range.)
+// The running maximum m of a row is that of s_j + log2(vs_j), with 2^log2(vs) the power of two above a key's value scale, rounded up to a whole number (all
+// factors between blocks and pieces are powers of two then). Weights times scales never exceed one against it, and the largest of them is at least 2^-6, however
+// much the scales of pages differ and whatever scales pages have that the row does not see or gives no weight. The sum of the weights without their
+// scales may lie as far from m as scales reach, 2^+-250.
+// The ordinary walk over a tile's blocks takes one power for the value scales of a block, so that the sum follows from the weighted weights, and a float for the
+// sum. That is good while the scales of a block lie within 2^4 of each other, and all of them within 2^30 of the last page's, which is their unit (and not below 2^-110). A warp that
+// meets others begins its part of the tile anew in a careful walk, where the sum has a power of two beside it and a block is gone through once for each 2^4 that its
+// scales span. (One walk for both issued 14 % more instructions: 64 requests of 2,048 keys 64 us instead of 61.)
 //
 // The work is a row of items, one for each block of 32 keys of each tile (rows of queries of one KV head) of each request, and every warp of the
 // grid takes an equal stretch of it, so that requests of any lengths keep all of them busy to the end; the boundaries are worked out on the GPU, from
@@ -26,6 +31,7 @@
 // is reading the cache: 2 D bytes per key and KV head. 64 requests of 2,048 keys, 32 / 8 heads of 128: 54 us (5.0 TB/s, 0.76 of measured) and 5 for
 // the join; the rest is the latency of a warp's chain of conversions, products and softmax at the twelve warps that an SM's registers hold.
 #include <cuda_fp16.h>
+#include <type_traits>
 
 #include "tma.cuh"
 
@@ -49,7 +55,8 @@ constexpr int TENSOR_BYTES = KEYS * D;
 constexpr int STAGE_BYTES = 2 * TENSOR_BYTES;      // a multiple of 1,024: swizzled panels start where the pattern does
 constexpr int SCALE_BYTES = 2 * KEYS * 4;
 constexpr int KSTEPS = D / 16;
-constexpr float P_FACTOR = 32768.f;            // weights are kept as 2^15 w
+constexpr float P_LOG2 = 15.f;                 // weights are kept as 2^15 w
+constexpr int NO_SCALE = -300;                 // stands for log2 of a scale of zero
 constexpr int GROUPS = 2 * THREADS, GROUP_BYTES = (GROUPS + 2 + WARPS) * 8;   // see Items
 // Of a kernel whose tiles have 8 NQ rows, (token, query head) pairs of one KV head:
 template <typename T, int NQ> struct Shape {
@@ -64,7 +71,7 @@ template <typename T, int NQ> struct Shape {
     static constexpr int STAGES = FIT < 4 ? FIT : 4;
     static_assert(STAGES >= 2, "room for a ring");
     static constexpr int RING_BYTES = WARPS * STAGES * STAGE_BYTES;
-    static constexpr int AT_BARS = RING_BYTES + WARPS * STAGES * SCALE_BYTES, AT_GROUPS = AT_BARS + WARPS * STAGES * 8, AT_Q = AT_GROUPS + GROUP_BYTES;
+    static constexpr int AT_BARS = RING_BYTES + WARPS * STAGES * SCALE_BYTES, AT_GROUPS = AT_BARS + WARPS * STAGES * 8, AT_POWERS = AT_GROUPS + GROUP_BYTES, AT_Q = AT_POWERS + THREADS * 2 * NQ * 2;
     static constexpr size_t SMEM = AT_Q + (Q_IN_REGS ? 0 : WARPS * Q_WORDS * 128);
     static_assert(SMEM <= 227 * 1024, "shared memory of a block");
 };
@@ -118,18 +125,47 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
 }
 __device__ __forceinline__ void store2(float* p, float2 v) { *reinterpret_cast<float2*>(p) = v; }
 __device__ __forceinline__ void store2(__nv_bfloat16* p, float2 v) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v.x, v.y); }
-// (top, total, v) += another maximum, sum and its entries. A sum of nothing has neither; a NaN may have a sum without a maximum and stays.
-template <int PER> __device__ __forceinline__ void add_piece(float& top, float& total, float4 (&v)[PER], float2 ml, const float4 (&u)[PER]) {
-    if (ml.y == 0.f) return;
-    const float n = fmaxf(top, ml.x), f0 = top == n ? 1.f : exp2_of(top - n), f1 = ml.x == n ? 1.f : exp2_of(ml.x - n);
-    top = n;
-    total = total * f0 + ml.y * f1;
-#pragma unroll
-    for (int x = 0; x < PER; ++x) {
-        v[x].x = v[x].x * f0 + u[x].x * f1; v[x].y = v[x].y * f0 + u[x].y * f1;
-        v[x].z = v[x].z * f0 + u[x].z * f1; v[x].w = v[x].w * f0 + u[x].w * f1;
-    }
+// A sum of weights, times 2^k. k is 0 unless the sum lies further than 2^30 from 1 (and it does not come near the ends of a float).
+struct Sum { float f; int k; };
+__device__ __forceinline__ double whole_of(const Sum& s) { return (double)s.f * __hiloint2double((1023 + max(s.k, -1022)) << 20, 0); }
+__device__ __forceinline__ Sum sum_of(double x) {
+    const int e = (__double2hiint(x) >> 20 & 0x7ff) - 1023;
+    if (e < -1000 || e > 1000 || abs(e) <= 30) return {(float)x, 0};      // 0, NaN, infinity; what a float holds well
+    return {(float)__hiloint2double(__double2hiint(x) - (e << 20), __double2loint(x)), e};
 }
+// What a row's sums are relative to, and the sum of its weights; of nothing: -inf and 0. A sum with a power of two beside it has a minus sign. (A NaN may have
+// a sum without a maximum.)
+struct __align__(8) RowSum { float m, total; };
+// (s, v) += N pieces of a row, powers left aside.
+template <int N> __device__ __forceinline__ void add_pieces(RowSum& s, float4& v, const RowSum (&y)[N], const float4 (&u)[N]) {
+    float n = s.m;
+    bool powers = s.total < 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) { n = fmaxf(n, y[i].m); powers |= y[i].total < 0.f; }
+    const float f0 = s.m == n ? 1.f : exp2_of(s.m - n);
+    float total = fabsf(s.total) * f0, f[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        f[i] = y[i].m == n ? 1.f : exp2_of(y[i].m - n);
+        total += fabsf(y[i].total) * f[i];
+    }
+    v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (y[i].total == 0.f) continue;
+        v.x += u[i].x * f[i]; v.y += u[i].y * f[i]; v.z += u[i].z * f[i]; v.w += u[i].w * f[i];
+    }
+    s = {n, powers ? -1.f : total};
+}
+// x * 2^e, by way of two powers: they, and what comes between, stay in range where the result does.
+struct Power { float a, b; };
+__device__ __forceinline__ Power power_of(float e) {
+    const float half = floorf(0.5f * e);
+    return {exp2_of(half), exp2_of(e - half)};
+}
+__device__ __forceinline__ float times(float x, const Power& p) { return x * p.a * p.b; }
+// What a row's sums are multiplied by at the end, 2^(base_exp - 15) / total.
+__device__ __forceinline__ Power final_unit(const Sum& total, int base_exp) { return power_of((float)(base_exp - total.k) - P_LOG2); }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -238,7 +274,8 @@ struct Cut {         // what the join has to know of a tile that a stretch ends 
 };
 struct Pieces {
     float* sums;     // [2 * warps][ROWS][D]
-    float2* ml;      // [2 * warps][ROWS] running maximum and sum
+    RowSum* rows;    // [2 * warps][ROWS]
+    int* powers;     // [2 * warps][ROWS], of sums that have one
     Cut* cuts;       // [warps]
 };
 
@@ -279,7 +316,10 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
     int turn = 0;      // stages filled before this tile: the ring and its barriers go on from there
     Cut cut = {-1, 0, 0, 0, 0, 0, {0, 0}};
 
-    for (int item = (int)min(all, (long long)me * share); item < end;) {
+    // The items from `item` on: where it came to, -1 if a wait ran out. An ordinary walk comes to `end` or to a tile whose scales it is not for.
+    auto stretch = [&](int item, auto careful) -> int {
+    constexpr bool CAREFUL = decltype(careful)::value;
+    while (item < end) {
     const Items::Place at = items.find(item);
     const int count = min(end - item, at.of.blocks - at.block);   // items of this tile that are this warp's
     item += count;
@@ -366,13 +406,17 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
         }
         cp_async_commit();
     };
-    int next_page = page_for(0);
+    int next_page;
+    auto prime = [&] {
+        next_page = page_for(0);
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-        const int page = next_page;
-        next_page = page_for(i + 1);
-        fetch(i, page);
-    }
+        for (int i = 0; i < STAGES - 1; ++i) {
+            const int page = next_page;
+            next_page = page_for(i + 1);
+            fetch(i, page);
+        }
+    };
+    prime();
 
     // ---- the queries: lane (g, quad) holds entries 16 c + 4 quad .. + 3 of rows g, g + 8, ...
     uint32_t q_regs[S::Q_IN_REGS ? S::Q_WORDS : 1];
@@ -381,7 +425,8 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
         else q_smem[word * 32 + lane] = v;      // (a lane reads what it has written)
     };
     float row_factor[NQ][2];       // of rows 2 quad and 2 quad + 1, as the scores come
-    int row_pos[NQ][2];
+    uint32_t row_toks = 0u;        // the tokens of rows 2 quad and 2 quad + 1 of each eight, a byte each
+    auto row_pos = [&](int nq, int e) { return first_pos + (int)(row_toks >> 8 * (2 * nq + e) & 255u); };
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
         const int r = g + 8 * nq, tok = r / a.heads_per_tile, head = hg * a.heads_per_tile + r % a.heads_per_tile;
@@ -414,7 +459,7 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             row_factor[nq][e] = __shfl_sync(0xffffffffu, factor, (2 * quad + e) * 4);
-            row_pos[nq][e] = first_pos + (8 * nq + 2 * quad + e) / a.heads_per_tile;
+            row_toks |= (uint32_t)__shfl_sync(0xffffffffu, tok, (2 * quad + e) * 4) << 8 * (2 * nq + e);
         }
     }
     auto get_q = [&](int word) -> uint32_t {
@@ -425,7 +470,9 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
 
     // sums: o[nq][m] holds entries 16 m + 2 g (words 0, 1) and 16 m + 2 g + 1 (words 2, 3) of rows 2 quad and 2 quad + 1
     float o[NQ][KSTEPS][4];
-    float m[NQ][2], l[NQ][2];
+    float m[NQ][2];
+    float l[NQ][2];
+    short* sum_k = reinterpret_cast<short*>(smem + S::AT_POWERS) + threadIdx.x * 2 * NQ;     // [NQ][2] a careful walk's powers of two of the sums
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
@@ -434,18 +481,26 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
             for (int e = 0; e < 4; ++e) o[nq][i][e] = 0.f;
         m[nq][0] = m[nq][1] = -INFINITY;
         l[nq][0] = l[nq][1] = 0.f;
+        if constexpr (CAREFUL) sum_k[2 * nq] = sum_k[2 * nq + 1] = 0;
     }
 
+    // the blocks from `first` up to `end`, which are on their way, arrive: before the stages are another's
+    auto arrived = [&](int first, int end) {
+        bool all = true;
+        if constexpr (TMA)
+            for (int k = first; k < min(end, mine); ++k) all = mbar_wait(bars + (turn + k) % STAGES, ((turn + k) / STAGES) & 1) && all;
+        cp_async_wait<0>();
+        return all;
+    };
     // ---- the walk
+    [[maybe_unused]] int top_exp = -(1 << 20);      // the largest value scale so far, as the power above it
     for (int i = 0; i < mine; ++i) {
         cp_async_wait<STAGES - 2>();
         const int slot = (turn + i) % STAGES;
         if (TMA && !mbar_wait(bars + slot, ((turn + i) / STAGES) & 1)) {
-            // what is on its way has to arrive before the block's memory is another's; nothing of this stretch is to be joined
-            if (lane == 0) { oxr_report(a.status, OXR_WAIT_EXPIRED, 40); left.cuts[me].last = -1; }
-            for (int k = i + 1; k < min(i + STAGES, mine); ++k) mbar_wait(bars + (turn + k) % STAGES, ((turn + k) / STAGES) & 1);
-            cp_async_wait<0>();
-            return;
+            if (lane == 0) oxr_report(a.status, OXR_WAIT_EXPIRED, 40);
+            arrived(i + 1, i + STAGES - 1);
+            return -1;
         }
         __syncwarp();
         {   // the stage that the block before this one has left
@@ -457,18 +512,26 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
         const float* scales = reinterpret_cast<const float*>(smem + SCALES_AT + (warp * STAGES + slot) * SCALE_BYTES);
         unsigned char* values = smem + (st - smem_addr(smem)) + TENSOR_BYTES;
         const int key0 = (block0 + i) * KEYS;
+        const uint32_t seen = __ballot_sync(0xffffffffu, key0 + lane >= lo && key0 + lane < hi);      // by any row
         if constexpr (TMA) {
             // Values that no row sees but that lie in a piece which one does, or in one that was not fetched, become zero: a weight of zero does not
             // undo a NaN. (Their scores are masked whatever the keys hold.)
-            const bool seen = key0 + lane >= lo && key0 + lane < hi;
-            if (__any_sync(0xffffffffu, !seen) || bad_page) {
-                if (!seen || bad_page) {
+            if (seen != 0xffffffffu || bad_page) {
+                if (!(seen >> lane & 1u) || bad_page) {
 #pragma unroll
                     for (int c = 0; c < KSTEPS; ++c) *reinterpret_cast<uint4*>(values + c / (PW / 16) * KEYS * PW + lane * PW + c % (PW / 16) * 16) = make_uint4(0, 0, 0, 0);
                 }
                 __syncwarp();
             }
         }
+
+        const uint32_t my_vs = __float_as_uint(scales[KEYS + lane]) & 0x7fffffffu;
+        uint32_t left_keys = seen;       // to be gone through
+        const bool whole = key0 >= last_lo && key0 + KEYS - 1 <= min(first_pos, hi - 1);
+        do {
+        // (asked for here, looked at behind the scores)
+        const bool is_left = left_keys >> lane & 1u;
+        const uint32_t most_vs = __reduce_max_sync(0xffffffffu, is_left ? my_vs : 0u), least_vs = __reduce_min_sync(0xffffffffu, is_left ? my_vs : 0xffffffffu);
 
         // scores: two tiles of 16 keys by 8 rows; c[..][mt]: key 16 mt + g (words 0, 1) and + 8 (words 2, 3) of rows 2 quad and 2 quad + 1
         float c[NQ][2][4];
@@ -501,21 +564,40 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
                 }
             }
         }
-        // the largest value scale of the block as a power of two, relative to the last page's
-        const float my_vs = scales[KEYS + lane];
-        const uint32_t most_vs = __reduce_max_sync(0xffffffffu, (my_vs > 0.f && my_vs < INFINITY) ? __float_as_uint(my_vs) : 0u);
-        const int lv = most_vs ? scale_exponent(__uint_as_float(most_vs)) - base_exp : 0;
+        // 2^lv: the power above the largest value scale, relative to the last page's scale; `now`: the keys whose scales lie within 2^4 of it
+        const bool finite = most_vs < 0x7f800000u;
+        const int most_exp = finite ? scale_exponent(__uint_as_float(most_vs)) : base_exp, lv = most_vs ? most_exp - base_exp : NO_SCALE;
+        uint32_t now = left_keys;
+        if constexpr (!CAREFUL) {
+            if (!finite || least_vs == 0u || most_vs - least_vs > 4u << 23 || lv > 30 || lv < -30 || most_exp < -110) {
+                const bool all = arrived(i + 1, i + STAGES);
+                if (!all && lane == 0) oxr_report(a.status, OXR_WAIT_EXPIRED, 40);
+                fence_proxy_async();
+                __syncwarp();
+                turn += min(mine, i + STAGES);
+                return all ? item - count : -1;
+            }
+            left_keys = 0u;
+        } else {
+            now = __ballot_sync(0xffffffffu, is_left && (finite ? (my_vs > 0u || most_vs == 0u) && most_vs - my_vs <= 4u << 23 : my_vs >= 0x7f800000u));
+            left_keys &= ~now;
+            if (finite) top_exp = max(top_exp, lv);
+        }
         const float lvf = (float)lv;
-        const float v_inverse = exp2_of(-(float)(lv + base_exp)), down = exp2_of(-lvf);
-        const bool whole = key0 >= last_lo && key0 + KEYS - 1 <= min(first_pos, hi - 1);
         float ks[4], vf[4];     // of keys g, g + 8, g + 16, g + 24
+        [[maybe_unused]] const float inverse = exp2_of(P_LOG2 - (float)most_exp);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             ks[j] = scales[g + 8 * j];
-            vf[j] = scales[KEYS + g + 8 * j] * v_inverse * P_FACTOR;   // at most 2^15
+            const float vs = scales[KEYS + g + 8 * j];
+            if constexpr (!CAREFUL) vf[j] = vs * inverse;      // at most 2^15
+            else vf[j] = now >> (8 * j + g) & 1u ? times(vs, power_of(P_LOG2 - (float)most_exp)) : 0.f;
         }
-        bool odd_scale = false;
-        if (!whole && tokens > 1) odd_scale = __any_sync(0xffffffffu, !(fabsf(my_vs) < INFINITY));
+        [[maybe_unused]] const float down = CAREFUL ? 0.f : exp2_of(-lvf);
+        auto hidden = [&](int nq, int e, int j) {       // key g + 8 j to row 2 quad + e
+            const int key = key0 + 8 * j + g, pos = row_pos(nq, e);
+            return !(now >> (8 * j + g) & 1u) || key > pos || (a.window > 0 && key <= pos - a.window);
+        };
         uint32_t p[NQ][PIECES][2][2];    // weights: [..][key tile][keys 0-7 or 8-15 of it]
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
@@ -527,39 +609,49 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
                     float& s = c[nq][j >> 1][(j & 1) * 2 + e];
                     s *= row_factor[nq][e] * ks[j];
                 }
-            if (!whole) {
+            if (CAREFUL || !whole) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int e = 0; e < 2; ++e)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int key = key0 + 8 * j + g;
-                        if (key > row_pos[nq][e] || (a.window > 0 && key <= row_pos[nq][e] - a.window) || key >= hi) c[nq][j >> 1][(j & 1) * 2 + e] = -INFINITY;
-                    }
+                    for (int j = 0; j < 4; ++j)
+                        if (hidden(nq, e, j)) c[nq][j >> 1][(j & 1) * 2 + e] = -INFINITY;
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) mx[e] = fmaxf(mx[e], c[nq][j >> 1][(j & 1) * 2 + e]);
             bool raise = false;
-            float n[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
-                n[e] = fmaxf(m[nq][e], mx[e] + lvf);
-                raise |= n[e] > m[nq][e];
+                raise |= mx[e] + lvf > m[nq][e];
             }
             if (__any_sync(0xffffffffu, raise)) {
-                const float a0 = n[0] > m[nq][0] ? exp2_of(m[nq][0] - n[0]) : 1.f, a1 = n[1] > m[nq][1] ? exp2_of(m[nq][1] - n[1]) : 1.f;
-                l[nq][0] *= a0; l[nq][1] *= a1;
 #pragma unroll
-                for (int x = 0; x < KSTEPS; ++x) { o[nq][x][0] *= a0; o[nq][x][1] *= a1; o[nq][x][2] *= a0; o[nq][x][3] *= a1; }
-                m[nq][0] = n[0]; m[nq][1] = n[1];
+                for (int e = 0; e < 2; ++e) {
+                    const float n = fmaxf(m[nq][e], ceilf(mx[e] + lvf)), f = n > m[nq][e] ? exp2_of(m[nq][e] - n) : 1.f;
+                    if (!CAREFUL) l[nq][e] *= f;
+                    else if (n > m[nq][e]) sum_k[2 * nq + e] = (short)max(sum_k[2 * nq + e] + (int)fmaxf(m[nq][e] - n, -2000.f), -2000);
+#pragma unroll
+                    for (int x = 0; x < KSTEPS; ++x) { o[nq][x][e] *= f; o[nq][x][2 + e] *= f; }
+                    m[nq][e] = n;
+                }
             }
             // weights: exp2(s - m) carries 2^lv into the products and none of it into the sum
             float off[2], sum[2] = {0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < 2; ++e) off[e] = m[nq][e] == -INFINITY ? 0.f : lvf - m[nq][e];
+            [[maybe_unused]] int up[2] = {-lv, -lv};
+            if (CAREFUL && lv < top_exp - 60) {
+                // a row may have met products to which these add nothing, although their weights count: those are taken by themselves
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (mx[e] > -INFINITY && mx[e] + off[e] < -60.f) {
+                        off[e] = -ceilf(mx[e]);
+                        up[e] = (int)fmaxf(-off[e] - m[nq][e], -1000.f);
+                    }
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -567,20 +659,21 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
                     float& w = c[nq][j >> 1][(j & 1) * 2 + e];
                     w = exp2_of(w + off[e]);
                     sum[e] += w;
+                    w *= vf[j];
                 }
-            if (odd_scale) {   // a hidden key's scale may be anything
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& w = c[nq][j >> 1][(j & 1) * 2 + e];
-                        w = w == 0.f ? 0.f : w * vf[j];
-                    }
+            if constexpr (!CAREFUL) {
+                l[nq][0] += sum[0] * down;
+                l[nq][1] += sum[1] * down;
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) c[nq][j >> 1][(j & 1) * 2 + e] *= vf[j];
+                    for (int j = 0; j < 4; ++j)
+                        if (up[e] != -lv || hidden(nq, e, j)) c[nq][j >> 1][(j & 1) * 2 + e] = 0.f;      // (a hidden key's scale may be anything)
+                    const Sum all = sum_of(whole_of({l[nq][e], sum_k[2 * nq + e]}) + whole_of({sum[e], up[e]}));
+                    l[nq][e] = all.f;
+                    sum_k[2 * nq + e] = (short)all.k;
+                }
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -589,8 +682,6 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
                 p[nq][0][j >> 1][j & 1] = transposed(packed);
                 if constexpr (PIECES == 2) p[nq][PIECES - 1][j >> 1][j & 1] = transposed(pack_rest(w0, w1, packed));
             }
-            l[nq][0] += sum[0] * down;
-            l[nq][1] += sum[1] * down;
         }
 
         // o += values x weights. Lanes 0-7 and 8-15 of an ldmatrix name keys 0-7 and 8-15 of a tile at 16-byte word n, lanes 16-31 the same keys at word
@@ -653,11 +744,12 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
                         }
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (row_pos[nq][e & 1] == pos) o[nq][n][e] += sum[e];
+                            if (row_pos(nq, e & 1) == pos) o[nq][n][e] += sum[e];
                     }
                 }
             }
         }
+        } while (CAREFUL && left_keys);
         fence_proxy_async();   // every lane has read the stage before the next turn's copies fill it
         __syncwarp();
     }
@@ -667,26 +759,36 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
     const bool whole_tile = at.block == 0 && count == at.of.blocks;
     if (at.block == 0 && !whole_tile)
         cut = {(item - count + at.of.blocks - 1) / share, q_begin + tok0, kvh * G + hg * a.heads_per_tile, rows, min(a.heads_per_tile, G - hg * a.heads_per_tile), base_exp, {0, 0}};
-    const float unscale = exp2_of((float)base_exp);
     const size_t place = (size_t)2 * me + (at.block == 0 ? 1 : 0);
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+            Sum total = {l[nq][e], 0};      // (every lane of a row has the same m)
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) l[nq][e] += __shfl_xor_sync(0xffffffffu, l[nq][e], x);
+            for (int x = 4; x < 32; x <<= 1) total.f += __shfl_xor_sync(0xffffffffu, total.f, x);
+            if constexpr (CAREFUL) {
+                double all = whole_of({l[nq][e], sum_k[2 * nq + e]});
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) all += __shfl_xor_sync(0xffffffffu, all, x);
+                total = sum_of(all);
+            }
             const int r = 8 * nq + 2 * quad + e, tok = r / a.heads_per_tile, head = hg * a.heads_per_tile + r % a.heads_per_tile;
             if (r >= rows || head >= G) continue;
-            const float total = l[nq][e];
             if (whole_tile) {
-                const float f = (1.f / P_FACTOR) / total;
+                const bool none = total.f == 0.f;
+                const Power unit = final_unit(total, base_exp);
+                const float f = 1.f / total.f * unit.a;
                 T* row = out + ((size_t)(q_begin + tok0 + tok) * a.H + (size_t)kvh * G + head) * D + 2 * g;
 #pragma unroll
                 for (int n = 0; n < KSTEPS; ++n)
-                    store2(row + 16 * n, total == 0.f ? make_float2(0.f, 0.f) : make_float2(o[nq][n][e] * f * unscale, o[nq][n][2 + e] * f * unscale));
+                    store2(row + 16 * n, none ? make_float2(0.f, 0.f) : make_float2(o[nq][n][e] * f * unit.b, o[nq][n][2 + e] * f * unit.b));
             } else {
                 // (all pieces of a tile are relative to the same scale)
-                if (g == 0) left.ml[place * ROWS + r] = make_float2(m[nq][e], total);
+                if (g == 0) {
+                    left.rows[place * ROWS + r] = {m[nq][e], total.k != 0 ? -total.f : fabsf(total.f)};
+                    if (total.k != 0) left.powers[place * ROWS + r] = total.k;
+                }
                 float* row = left.sums + (place * ROWS + r) * D + 2 * g;
 #pragma unroll
                 for (int n = 0; n < KSTEPS; ++n) *reinterpret_cast<float2*>(row + 16 * n) = make_float2(o[nq][n][e], o[nq][n][2 + e]);
@@ -694,17 +796,24 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
         }
     __syncwarp();
     }
-    if (lane == 0) left.cuts[me] = cut;
+    return item;
+    };
+    int item = stretch((int)min(all, (long long)me * share), std::false_type{});
+    if (item >= 0 && item < end) item = stretch(item, std::true_type{});
+    if (lane == 0) {
+        if (item < 0) cut.last = -1;      // nothing of this stretch is to be joined
+        left.cuts[me] = cut;
+    }
 }
 
 // Joins the pieces of the tiles that lie in more than one warp's stretch. A block looks at some of the stretches and, of each that ends in a tile
 // which began in it, takes eight rows of the tile. A thread has four entries of a row; where the rows leave threads over, they take the pieces in turn.
 constexpr int JOIN_THREADS = 256, JOIN_ROWS = D <= 128 ? 8 : 4, JOIN_BLOCKS = 592;
 template <typename T, int NQ>
-__global__ void __launch_bounds__(JOIN_THREADS) attn_kv8_join_kernel(T* __restrict__ out, const Pieces left, const int warps, const int H, const int heads_per_tile) {
+__global__ void __launch_bounds__(JOIN_THREADS, 3) attn_kv8_join_kernel(T* __restrict__ out, const Pieces left, const int warps, const int H, const int heads_per_tile) {
     constexpr int ROWS = 8 * NQ, WORDS = D / 4;
     __shared__ float4 sums[JOIN_THREADS];
-    __shared__ float2 ml[JOIN_THREADS];
+    __shared__ RowSum rows[JOIN_THREADS];
     pdl_wait();
     pdl_trigger();
     const int lane = threadIdx.x & 31, r0 = (int)blockIdx.y * JOIN_ROWS;
@@ -719,39 +828,53 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_kv8_join_kernel(T* __restri
             int ways = 1;      // threads that share an entry's pieces
             while (ways * 2 * all <= JOIN_THREADS) ways *= 2;
             const int x = threadIdx.x % all, way = threadIdx.x / all, r = r0 + x / WORDS, d = x % WORDS * 4;
-            float top = -INFINITY, total = 0.f;
-            float4 v[1] = {make_float4(0.f, 0.f, 0.f, 0.f)};
+            RowSum s = {-INFINITY, 0.f};
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (way < ways) {
                 for (int p0 = first + way; p0 <= cut.last; p0 += 8 * ways) {     // eight pieces at a time
-                    float2 y[8];
-                    float4 u[8][1];
+                    RowSum y[8];
+                    float4 u[8];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const int w = p0 + k * ways;
                         const size_t at = ((size_t)2 * w + (w == first ? 1 : 0)) * ROWS + r;
-                        y[k] = w <= cut.last ? __ldcg(left.ml + at) : make_float2(-INFINITY, 0.f);
-                        u[k][0] = w <= cut.last ? __ldcg(reinterpret_cast<const float4*>(left.sums + at * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        const float2 ml = w <= cut.last ? __ldcg(reinterpret_cast<const float2*>(left.rows + at)) : make_float2(-INFINITY, 0.f);
+                        y[k] = {ml.x, ml.y};
+                        u[k] = w <= cut.last ? __ldcg(reinterpret_cast<const float4*>(left.sums + at * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
                     }
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) add_piece<1>(top, total, v, y[k], u[k]);
+                    add_pieces(s, v, y, u);
                 }
             }
             if (ways > 1) {
-                sums[threadIdx.x] = v[0];
-                ml[threadIdx.x] = make_float2(top, total);
+                sums[threadIdx.x] = v;
+                rows[threadIdx.x] = s;
                 __syncthreads();
                 if (way == 0)
                     for (int k = 1; k < ways; ++k) {
+                        const RowSum y[1] = {rows[k * all + x]};
                         const float4 u[1] = {sums[k * all + x]};
-                        add_piece<1>(top, total, v, ml[k * all + x], u);
+                        add_pieces(s, v, y, u);
                     }
                 __syncthreads();
             }
             const int head = r % heads_per_tile;
             if (way == 0 && head < cut.heads) {
-                const float f = (1.f / P_FACTOR) / total, unscale = exp2_of((float)cut.base_exp);
-                float4 z = make_float4(v[0].x * f * unscale, v[0].y * f * unscale, v[0].z * f * unscale, v[0].w * f * unscale);
-                if (total == 0.f) z = make_float4(0.f, 0.f, 0.f, 0.f);
+                Sum total = {s.total, 0};
+                if (s.total < 0.f) {      // again, with the powers
+                    double all = 0.;
+#pragma unroll 1
+                    for (int w = first; w <= cut.last; ++w) {
+                        const size_t at = ((size_t)2 * w + (w == first ? 1 : 0)) * ROWS + r;
+                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(left.rows + at));
+                        const int k = ml.y < 0.f ? __ldcg(left.powers + at) : 0;
+                        all += whole_of({fabsf(ml.y), k + (ml.x == s.m ? 0 : (int)fmaxf(ml.x - s.m, -2000.f))});
+                    }
+                    total = sum_of(all);
+                }
+                const Power unit = final_unit(total, cut.base_exp);
+                const float f = 1.f / total.f * unit.a;
+                float4 z = make_float4(v.x * f * unit.b, v.y * f * unit.b, v.z * f * unit.b, v.w * f * unit.b);
+                if (total.f == 0.f) z = make_float4(0.f, 0.f, 0.f, 0.f);
                 store4(out + ((size_t)(cut.token + r / heads_per_tile) * H + cut.head + head) * D + d, z);
             }
         }
@@ -792,8 +915,9 @@ int launch(void* out, const void* q, const Kv8Args& a, int blocks, float* scratc
     const int code = tma ? allow<T, true, NQ>() : allow<T, false, NQ>();
     if (code != 0) return code;
     const int warps = blocks * WARPS;
-    float2* ml = reinterpret_cast<float2*>(scratch + (size_t)2 * warps * 8 * NQ * D);
-    const Pieces left = {scratch, ml, reinterpret_cast<Cut*>(ml + (size_t)2 * warps * 8 * NQ)};
+    RowSum* rows = reinterpret_cast<RowSum*>(scratch + (size_t)2 * warps * 8 * NQ * D);
+    int* powers = reinterpret_cast<int*>(rows + (size_t)2 * warps * 8 * NQ);
+    const Pieces left = {scratch, rows, powers, reinterpret_cast<Cut*>(powers + (size_t)2 * warps * 8 * NQ)};
     const dim3 grid(blocks), threads(THREADS);
     if (tma) oxr_launch(attn_kv8_kernel<T, true, NQ>, grid, threads, Shape<T, NQ>::SMEM, stream, true, (T*)out, (const T*)q, map_k, map_v, piece_shift, a, left);
     else oxr_launch(attn_kv8_kernel<T, false, NQ>, grid, threads, Shape<T, NQ>::SMEM, stream, true, (T*)out, (const T*)q, map_k, map_v, piece_shift, a, left);

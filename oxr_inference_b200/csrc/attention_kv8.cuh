@@ -46,7 +46,7 @@ struct Kv8Call {
     const int* cu_q;                // [n + 1]
     const int* ctx_lens;            // [n]
     const int* block_table;         // [n, table_width]
-    float* scratch;                 // of the split-key kernel: 8 * blocks * tile_rows * (D + 2) + 32 * blocks words
+    float* scratch;                 // of the split-key kernel: 8 * blocks * tile_rows * (D + 3) + 32 * blocks words
     int* status;
     cudaStream_t stream;
     long long page_stride, q_stride;

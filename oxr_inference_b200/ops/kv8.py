@@ -175,7 +175,7 @@ def _split_plan(requests: int, tokens: int, longest: int, group: int, kv: int, h
     per_tile = rows // heads_per_tile
     tiles = min(tokens, requests * -(-longest // per_tile), requests + tokens // per_tile) * kv * -(-group // heads_per_tile)
     blocks = kv8_blocks(tiles, -(-seen // 32), _kv8_room(head_dim, code, rows))
-    return rows, blocks, 8 * blocks * rows * (head_dim + 2) + 32 * blocks
+    return rows, blocks, 8 * blocks * rows * (head_dim + 3) + 32 * blocks
 
 
 @functools.lru_cache(maxsize=None)
