@@ -56,7 +56,6 @@ constexpr int STAGE_BYTES = 2 * TENSOR_BYTES;      // a multiple of 1,024: swizz
 constexpr int SCALE_BYTES = 2 * KEYS * 4;
 constexpr int KSTEPS = D / 16;
 constexpr float P_LOG2 = 15.f;                 // weights are kept as 2^15 w
-constexpr int NO_SCALE = -300;                 // stands for log2 of a scale of zero
 constexpr int GROUPS = 2 * THREADS, GROUP_BYTES = (GROUPS + 2 + WARPS) * 8;   // see Items
 // Of a kernel whose tiles have 8 NQ rows, (token, query head) pairs of one KV head:
 template <typename T, int NQ> struct Shape {
@@ -156,12 +155,6 @@ template <int N> __device__ __forceinline__ void add_pieces(RowSum& s, float4& v
         v.x += u[i].x * f[i]; v.y += u[i].y * f[i]; v.z += u[i].z * f[i]; v.w += u[i].w * f[i];
     }
     s = {n, powers ? -1.f : total};
-}
-// x * 2^e, by way of two powers: they, and what comes between, stay in range where the result does.
-struct Power { float a, b; };
-__device__ __forceinline__ Power power_of(float e) {
-    const float half = floorf(0.5f * e);
-    return {exp2_of(half), exp2_of(e - half)};
 }
 __device__ __forceinline__ float times(float x, const Power& p) { return x * p.a * p.b; }
 // What a row's sums are multiplied by at the end, 2^(base_exp - 15) / total.

@@ -8,6 +8,7 @@
 namespace {
 constexpr int D = HEAD_DIM;
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int NO_SCALE = -300;     // stands for log2 of a value scale of zero
 
 struct Kv8Args {
     const unsigned char* k_cache;
@@ -170,5 +171,11 @@ __device__ __forceinline__ float exp2_of(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// 2^e as the product of two powers: x * a * b, and what comes between, stays in range where the result does.
+struct Power { float a, b; };
+__device__ __forceinline__ Power power_of(float e) {
+    const float half = floorf(0.5f * e);
+    return {exp2_of(half), exp2_of(e - half)};
 }
 }  // namespace

@@ -7,16 +7,21 @@
 //     O += P V       tcgen05.mma with P from tensor memory.
 // kind::f8f6f4 would take the codes as they are, but its other operand would have to have 8 bits too, and two e4m3 numbers for each weight cost the
 // softmax threads more than what is done instead: seven warps turn the codes of a block, while it passes from global to shared memory, into fp16
-// numbers, times the ratio of their page's scale to the block's largest (a power of two when the scales are; the products are then exact). The block's
-// largest key scale goes into the factor of the scores, the largest value scale as its logarithm into the exponent of the weights, so that
-// neither costs the softmax an instruction per key. Weights are kept as 2^7 P against a maximum that is raised in steps of 2^8: below 2^15 in
-// fp16, with their eleven bits down to 2^-21 of the largest.
+// numbers, times the ratio of their scale to the block's largest where that is a power of two and the products are exact: for keys from 2^-14 on, for values
+// from 2^-4 on, which leaves the weights their bits; elsewhere times 1. In an even block that is so of all keys (and the largest value scale within 2^60 of the last
+// page's), as it mostly is among the store's scales: the largest key scale goes into the factor of the scores, the largest value scale, as its logarithm, into the exponent of
+// the weights, and neither costs the softmax an instruction per key. In other blocks (and in one whose value scales are 2^60 below some met before) the softmax
+// takes keys one by one, each with its own scales. As in the split-key kernel the maximum is that of score and value scale, in whole numbers, and the sum of
+// the weights a double: a row's result does not hang on scales that it does not see or gives no weight.
+// Weights are kept as 2^7 P against a maximum that is raised in steps of 2^8: below 2^15 in
+// fp16, with their eleven bits down to 2^-21 of the largest (2^-17 in an even block).
 // Warps: 0 issues the products and owns the tensor memory, 1 to 3 and 12 to 15 bring in keys and values, 4 to 7 and 8 to 11 are the
 // softmax of the first and the second half; setmaxnreg gives those 160 registers (128 scores and what goes with them) and the others 96 (with 64 the
 // codes on their way were spilled: 404 us instead of 146 in the case below).
 // What bounds it: per block of 128 keys the products take 2,048 cycles of the tensor pipe and about as much shared-memory bandwidth, the exponentials 2,048 of
-// theirs. 2,048 tokens on 2,048 cached ones, 32 / 8 heads of 128, take 144 us (714 TFLOP/s, 0.44 of measured): 2.9 us a block. Without the loaders' work it would be 120,
-// without the softmax's arithmetic 133: two chains of latencies that are equally long and share the issue slots.
+// theirs. 2,048 tokens on 2,048 cached ones, 32 / 8 heads of 128, take 146 us (706 TFLOP/s, 0.43 of measured): 2.9 us a block. Without the loaders' work it would be 120,
+// without the softmax's arithmetic 133: two chains of latencies that are equally long and share the issue slots. With scales of any mantissa, every block of them
+// uneven, it takes 320.
 // Every wait on an mbarrier is bounded.
 #include <cuda_fp16.h>
 
@@ -43,10 +48,17 @@ constexpr float RAISE = 8.f;
 constexpr float P_SHIFT = 7.f;
 constexpr uint32_t TMEM_COLS = 512;                      // S | P of half h at 128 h, O of half h at 256 + h O_COLS
 
-struct BlockInfo {
-    long long row[KEYS];       // byte offset of each key's row in the pools; -1: zeros stand for it
+struct __align__(16) BlockInfo {
+    union {
+        long long row[KEYS];   // byte offset of each key's row in the pools; -1: zeros stand for it
+        float v_exp[KEYS];     // of an uneven block, once its codes have been asked for
+    };
+    // Scales; of an uneven block then what is left of them beside the ratios: a factor of a key's scores, and of its values a power of two, as its exponent
+    // relative to the last page's, and a factor of up to 1.
     float k_scale[KEYS], v_scale[KEYS];
+    __half2 k_ratio[KEYS], v_ratio[KEYS];   // what codes are multiplied by: a scale over the block's largest, or 1 where that is not exact
     float k_most[4], v_most[4];   // of each 32 keys: the largest scale
+    int even;                  // all of them are exact
     float factor, shift;       // of the block: its largest key scale; log2 of its largest value scale, relative to the last page's
 };
 struct Shared {
@@ -134,6 +146,94 @@ __device__ __forceinline__ bool has_nan(uint4 w) {
 }
 __device__ __forceinline__ float usable(float scale) { return scale > 0.f && scale < INFINITY ? scale : 0.f; }
 
+// A row's running maximum (see the head of the file; a whole number), and the sum of its weights 2^(score - m).
+struct Row {
+    float m;
+    double l;
+};
+// A block's largest score with its value scale is `mx`: the maximum is raised to it, if it is 2^RAISE above, and with it go the sums. By whole warps.
+__device__ __forceinline__ void raise_row(Row& row, float mx, uint32_t tmem_o, bool begun) {
+    float alpha = 1.f;
+    const bool raise = mx > row.m + RAISE || (row.m == -INFINITY && mx != -INFINITY);
+    if (raise) {
+        const float n = ceilf(mx);
+        alpha = row.m == -INFINITY ? 0.f : exp2_of(row.m - n);
+        row.l *= __hiloint2double((int)(fmaxf(row.m - n, -1022.f) + 1023.f) << 20, 0);
+        row.m = n;
+    }
+    // S(b) complete means that O += P(b - 1) V(b - 1), issued before it, is complete: O may be rescaled
+    if (__any_sync(0xffffffffu, raise && begun)) {
+#pragma unroll 1
+        for (int c = 0; c < D / 16; ++c) {
+            uint32_t ov[16];
+            ld16(tmem_o + (uint32_t)(c * 16), ov);
+            wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * alpha);
+            st16(tmem_o + (uint32_t)(c * 16), ov);
+        }
+        wait_st();
+    }
+}
+// The softmax of an uneven block, key by key; a row sees keys row_lo .. row_pos. By whole warps. (A function of its own: inlined it took registers from the ordinary
+// block's softmax.)
+__device__ __noinline__ Row one_by_one(const BlockInfo& f, uint32_t tmem_s, uint32_t tmem_o, float row_factor, int key0, int row_lo, int row_pos, bool begun, Row row) {
+    // The scores of 32 keys, the hidden ones' -inf.
+    auto scores_of = [&](int c, float (&x)[32]) {
+        uint32_t v[32];
+        ld32(tmem_s + (uint32_t)(c * 32), v);
+        const int low = max(row_lo - key0 - c * 32, 0), high = min(row_pos - key0 - c * 32, 31);      // the first and the last that the row sees
+        const uint32_t seen = row_pos >= row_lo && low <= high ? (0xffffffffu >> (31 - high)) & (0xffffffffu << low) : 0u;
+        wait_ld();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 k = reinterpret_cast<const float4*>(f.k_scale)[c * 8 + i];
+            const float kp[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[4 * i + j] = seen >> (4 * i + j) & 1u ? __uint_as_float(v[4 * i + j]) * (row_factor * kp[j]) : -INFINITY;
+        }
+    };
+    float mx = -INFINITY, sc = -INFINITY;      // the largest score + log2 of the value scale; the largest score
+#pragma unroll 1
+    for (int c = 0; c < KEYS / 32; ++c) {
+        float x[32];
+        scores_of(c, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 e = reinterpret_cast<const float4*>(f.v_exp)[c * 8 + i];
+            sc = fmaxf(max3(sc, x[4 * i], x[4 * i + 1]), fmaxf(x[4 * i + 2], x[4 * i + 3]));
+            mx = fmaxf(max3(mx, x[4 * i] + e.x, x[4 * i + 1] + e.y), fmaxf(x[4 * i + 2] + e.z, x[4 * i + 3] + e.w));
+        }
+    }
+    raise_row(row, mx, tmem_o, begun);
+    const float most = sc == -INFINITY ? 0.f : ceilf(sc), off = (row.m == -INFINITY ? 0.f : -row.m) + P_SHIFT;
+    float sum = 0.f;
+#pragma unroll 1
+    for (int c = 0; c < KEYS / 32; ++c) {      // (the columns that 32 weights go to held scores that have been read)
+        float x[32];
+        uint32_t pv[16];
+        scores_of(c, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 e4 = reinterpret_cast<const float4*>(f.v_exp)[c * 8 + i], p4 = reinterpret_cast<const float4*>(f.v_scale)[c * 8 + i];
+            const float e[4] = {e4.x, e4.y, e4.z, e4.w}, p[4] = {p4.x, p4.y, p4.z, p4.w};
+            float w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float y = x[4 * i + j];
+                sum += exp2_of(y - most);
+                w[j] = y == -INFINITY ? 0.f : exp2_of(y + (e[j] + off)) * p[j];      // (a hidden key's scale may be anything)
+            }
+            const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
+            pv[2 * i] = *reinterpret_cast<const uint32_t*>(&h0);
+            pv[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+        }
+        st16(tmem_s + (uint32_t)(c * 16), pv);
+    }
+    if (sum != 0.f) row.l += (double)sum * __hiloint2double((int)(fminf(fmaxf(most - row.m, -1000.f), 1000.f) + 1023.f) << 20, 0);
+    return row;
+}
+
 __global__ void __launch_bounds__(THREADS, 1)
 attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ q, const Kv8Args a, const int tiles) {
     extern __shared__ __align__(1024) unsigned char smem[];     // nothing static stands before it
@@ -206,9 +306,10 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                 if (lt >= KEYS) return;
                 BlockInfo& f = sh.info[b % INFO];
                 const int key = (block0 + b) * KEYS + lt;
-                f.row[lt] = page >= 0 ? (long long)page * a.page_stride + a.row_in_page(key, kvh) : -1;
                 f.k_scale[lt] = ks;
                 f.v_scale[lt] = vs;
+                f.row[lt] = page >= 0 ? (long long)page * a.page_stride + a.row_in_page(key, kvh) : -1;
+                if (lt == 0) f.even = 1;
                 // (positive floats compare as integers do)
                 const uint32_t km = __reduce_max_sync(0xffffffffu, __float_as_uint(usable(ks))), vm = __reduce_max_sync(0xffffffffu, __float_as_uint(usable(vs)));
                 if (lane == 0) { f.k_most[lt / 32] = __uint_as_float(km); f.v_most[lt / 32] = __uint_as_float(vm); }
@@ -229,36 +330,32 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                     c[p] = row >= 0 ? __ldg(reinterpret_cast<const uint4*>(pool + row + col_of(p) * 16)) : make_uint4(0, 0, 0, 0);
                 }
             };
-            // A NaN that some row does not see is taken out here and put into the rows that see it at the end; likewise values whose scale is not finite.
-            auto take_out = [&](uint4 (&c)[PASSES], const float* scales) {
+            // A NaN that some row does not see is taken out here and put into the rows that see it at the end.
+            auto take_out = [&](uint4 (&c)[PASSES]) {
 #pragma unroll 1
                 for (int p = 0; p < PASSES; ++p) {
                     uint4 w = make_uint4(0, 0, 0, 0);
 #pragma unroll
                     for (int x = 0; x < PASSES; ++x)
                         if (x == p) w = c[x];
-                    const bool finite = key_of(p) >= KEYS || fabsf(scales[min(key_of(p), KEYS - 1)]) < INFINITY;
-                    if (finite && !has_nan(w)) continue;
+                    if (!has_nan(w)) continue;
                     sh.nan_values = 1;
-                    const uint32_t all = finite ? 0xffffffffu : 0u;
-                    w.x &= ~__vcmpeq4(w.x & 0x7f7f7f7fu, 0x7f7f7f7fu) & all;
-                    w.y &= ~__vcmpeq4(w.y & 0x7f7f7f7fu, 0x7f7f7f7fu) & all;
-                    w.z &= ~__vcmpeq4(w.z & 0x7f7f7f7fu, 0x7f7f7f7fu) & all;
-                    w.w &= ~__vcmpeq4(w.w & 0x7f7f7f7fu, 0x7f7f7f7fu) & all;
+                    w.x &= ~__vcmpeq4(w.x & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                    w.y &= ~__vcmpeq4(w.y & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                    w.z &= ~__vcmpeq4(w.z & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                    w.w &= ~__vcmpeq4(w.w & 0x7f7f7f7fu, 0x7f7f7f7fu);
 #pragma unroll
                     for (int x = 0; x < PASSES; ++x)
                         if (x == p) c[x] = w;
                 }
             };
             // The codes of a block as fp16 numbers, times the ratio of their scale to the block's largest, into a stage.
-            auto put = [&](const uint4 (&c)[PASSES], unsigned char* stage, const float* scales, float inverse, bool careful) {
+            auto put = [&](const uint4 (&c)[PASSES], unsigned char* stage, const __half2* ratios) {
 #pragma unroll
                 for (int p = 0; p < PASSES; ++p) {
                     const int key = key_of(p), col = col_of(p);
                     if (key >= KEYS) continue;
-                    float ratio = scales[key] * inverse;
-                    if (careful && !(fabsf(ratio) < INFINITY)) ratio = 0.f;
-                    const __half2 r = __float2half2_rn(ratio);
+                    const __half2 r = ratios[key];
                     unsigned char* dst = stage + (col >> 2) * PANEL_BYTES + key * 128;
                     // threads of the second panel begin with the second of their two 16-byte words: the eight of a key then write to different banks
                     const int second = (col >> 2) & 1;
@@ -278,14 +375,58 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                 fence_proxy_async();
                 __syncwarp();
             };
+            // A key's ratios, by its thread: a power of two of 2^-14 and more for keys and 2^-4 and more for values, else 1. (The mantissas are the same but for the
+            // rounding of the quotient.)
+            auto most_of = [&](const float (&m)[4]) { return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])); };
+            auto exact = [](float x, uint32_t least) {
+                const uint32_t bits = __float_as_uint(x) + 4u;
+                return bits - least <= 0x3f800008u - least && (bits & 0x7ffff0u) == 0u;
+            };
+            constexpr uint32_t K_LEAST = 0x38800000u, V_LEAST = 0x3d800000u;
+            float top = -1e9f;       // the largest of the blocks' shifts so far
+            auto put_ratios = [&](int b, int page, float ks, float vs) {
+                if (lt >= KEYS || b >= count) return;
+                BlockInfo& f = sh.info[b % INFO];
+                const float km = most_of(f.k_most), vm = most_of(f.v_most);
+                const float kr = __fdividef(ks, km), vr = __fdividef(vs, vm);
+                const bool k_exact = exact(kr, K_LEAST) || ks == 0.f, v_exact = exact(vr, V_LEAST);
+                f.k_ratio[lt] = __float2half2_rn(k_exact ? (ks == 0.f ? 0.f : kr) : 1.f);
+                f.v_ratio[lt] = __float2half2_rn(v_exact ? vr : 1.f);
+                const float shift = fmaxf(log2f(vm) - (float)base_exp, (float)NO_SCALE);
+                top = fmaxf(top, shift);
+                if (page >= 0 && !(k_exact && v_exact && fabsf(shift) <= 60.f && shift >= top - 60.f)) f.even = 0;
+                if (lt == 0) {
+                    f.factor = km > 0.f ? km : 1.f;
+                    f.shift = shift;
+                }
+            };
+            // What the softmax needs for the keys of an uneven block.
+            auto put_parts = [&](BlockInfo& f) {
+                const float km = most_of(f.k_most), vm = most_of(f.v_most), ks = f.k_scale[lt], vs = f.v_scale[lt];
+                if (exact(__fdividef(ks, km), K_LEAST)) f.k_scale[lt] = km;
+                if (exact(__fdividef(vs, vm), V_LEAST)) {
+                    f.v_exp[lt] = f.shift;
+                    f.v_scale[lt] = 1.f;
+                } else {
+                    const int up = fabsf(vs) < INFINITY ? scale_exponent(fabsf(vs)) : base_exp;
+                    const Power unit = power_of(-(float)up);
+                    f.v_exp[lt] = (float)(vs == 0.f ? NO_SCALE : up - base_exp);
+                    f.v_scale[lt] = vs * unit.a * unit.b;
+                }
+            };
+            // of the block behind the present one
             int page1 = page_for(1);
+            float ks1 = scale_of(a.k_scale, page1), vs1 = scale_of(a.v_scale, page1);
+            int page2 = page_for(2);
             {
                 const int page0 = page_for(0);
-                put_info(0, page0, scale_of(a.k_scale, page0), scale_of(a.v_scale, page0));
-                put_info(1, page1, scale_of(a.k_scale, page1), scale_of(a.v_scale, page1));
+                const float ks0 = scale_of(a.k_scale, page0), vs0 = scale_of(a.v_scale, page0);
+                put_info(0, page0, ks0, vs0);
+                put_info(1, page1, ks1, vs1);
+                loaders_meet();
+                put_ratios(0, page0, ks0, vs0);
+                loaders_meet();
             }
-            int page2 = page_for(2);
-            loaders_meet();
             ask(kc, a.k_cache, 0);
             ask(vc, a.v_cache, 0);
             bool ok = true;        // (a thread that has given up keeps meeting the others)
@@ -294,22 +435,19 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                 const int st = b % STAGES;
                 const float ks = scale_of(a.k_scale, page2), vs = scale_of(a.v_scale, page2);      // of block b + 2
                 const int page3 = page_for(b + 3);
-                const float km = fmaxf(fmaxf(f.k_most[0], f.k_most[1]), fmaxf(f.k_most[2], f.k_most[3]));
-                const float vm = fmaxf(fmaxf(f.v_most[0], f.v_most[1]), fmaxf(f.v_most[2], f.v_most[3]));
-                if (lt == 0) {
-                    f.factor = km > 0.f ? km : 1.f;
-                    f.shift = vm > 0.f ? log2f(vm) - (float)base_exp : 0.f;
-                }
+                if (lt < KEYS && !f.even) put_parts(f);      // (its rows have been asked for)
                 ok = ok && mbar_wait(sh.k_empty + st, ((b / STAGES) & 1) ^ 1);
-                put(kc, k_ring + st * TENSOR_BYTES, f.k_scale, km > 0.f ? 1.f / km : 1.f, false);
+                put(kc, k_ring + st * TENSOR_BYTES, f.k_ratio);
                 if (lane == 0) mbar_arrive(sh.k_full + st);
                 ask(kc, a.k_cache, b + 1);
                 ok = ok && mbar_wait(sh.v_empty + st, ((b / STAGES) & 1) ^ 1);
-                if (partial(b)) take_out(vc, f.v_scale);
-                put(vc, v_ring + st * TENSOR_BYTES, f.v_scale, vm > 0.f ? 1.f / vm : 1.f, partial(b));
+                if (partial(b)) take_out(vc);
+                put(vc, v_ring + st * TENSOR_BYTES, f.v_ratio);
                 if (lane == 0) mbar_arrive(sh.v_full + st);
                 ask(vc, a.v_cache, b + 1);
+                put_ratios(b + 1, page1, ks1, vs1);      // (here rather than at the loop's start, which delays the keys: 146 us instead of 150 in the case above)
                 put_info(b + 2, page2, ks, vs);
+                page1 = page2; ks1 = ks; vs1 = vs;
                 page2 = page3;
                 loaders_meet();
             }
@@ -394,75 +532,65 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
             if (lane == 0) mbar_arrive(&sh.q_ready);
         }
         if (half == 0 || half1_live) {
-            float m_used = -INFINITY, l = 0.f;      // of score + shift, in log2 units; the sum of 2^7 weights
+            Row row = {-INFINITY, 0.};
             bool alive = true;
             for (int b = 0; b < count; ++b) {
                 if (!mbar_wait(sh.s_full + half, b & 1)) { if (lane == 0) oxr_report(a.status, OXR_WAIT_EXPIRED, 46); alive = false; break; }
                 fence_after();
                 const int key0 = (block0 + b) * KEYS;
+                const BlockInfo& f = sh.info[b % INFO];
+                const bool even = f.even != 0;
                 // (never zero: a hidden score of -inf has to stay one)
-                const float factor = fmaxf(row_factor * sh.info[b % INFO].factor, 1e-37f), shift = sh.info[b % INFO].shift;
-                uint32_t sv[KEYS / 32][32];
-#pragma unroll
-                for (int c = 0; c < KEYS / 32; ++c) ld32(tmem_s + (uint32_t)(c * 32), sv[c]);
-                wait_ld();
+                const float factor = fmaxf(row_factor * f.factor, 1e-37f), shift = f.shift;
                 // Rows without a token or head see what comes (their queries are zero); the others see keys row_lo .. row_pos.
-                if (key0 < row_lo || key0 + KEYS - 1 > row_pos) {
-                    const int from = row_lo - key0;
-                    const unsigned span = row_pos >= row_lo ? (unsigned)(row_pos - row_lo) : 0u;
+                const bool some_hidden = key0 < row_lo || key0 + KEYS - 1 > row_pos;
+                const int from = row_lo - key0;
+                const unsigned span = row_pos >= row_lo ? (unsigned)(row_pos - row_lo) : 0u;
+                auto hidden = [&](int j) { return (unsigned)(j - from) > span || row_pos < row_lo; };
+                if (even) {
+                    uint32_t sv[KEYS / 32][32];
+#pragma unroll
+                    for (int c = 0; c < KEYS / 32; ++c) ld32(tmem_s + (uint32_t)(c * 32), sv[c]);
+                    wait_ld();
+                    if (some_hidden) {
+#pragma unroll
+                        for (int c = 0; c < KEYS / 32; ++c)
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (hidden(c * 32 + j)) sv[c][j] = __float_as_uint(-INFINITY);
+                    }
+                    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int c = 0; c < KEYS / 32; ++c)
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if ((unsigned)(c * 32 + j - from) > span || row_pos < row_lo) sv[c][j] = __float_as_uint(-INFINITY);
-                }
-                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        for (int j = 0; j < 16; ++j) mx4[j & 3] = max3(mx4[j & 3], __uint_as_float(sv[c][2 * j]), __uint_as_float(sv[c][2 * j + 1]));
+                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * factor + shift;
+                    raise_row(row, mx, tmem_o, b > 0);
+                    const float off = (row.m == -INFINITY ? 0.f : shift - row.m) + P_SHIFT;
+                    const uint64_t factor2 = pair_of(factor, factor), off2 = pair_of(off, off);
+                    uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-                for (int c = 0; c < KEYS / 32; ++c)
+                    for (int c = 0; c < KEYS / 32; ++c) {
+                        uint32_t pv[16];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) mx4[j & 3] = max3(mx4[j & 3], __uint_as_float(sv[c][2 * j]), __uint_as_float(sv[c][2 * j + 1]));
-                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * factor + shift;
-                float alpha = 1.f;
-                const bool raise = mx > m_used + RAISE || (m_used == -INFINITY && mx != -INFINITY);
-                if (raise) {
-                    alpha = m_used == -INFINITY ? 0.f : exp2_of(m_used - mx);
-                    m_used = mx;
-                }
-                // S(b) complete means that O += P(b - 1) V(b - 1), issued before it, is complete: O may be rescaled
-                if (__any_sync(0xffffffffu, raise && b > 0)) {
-#pragma unroll 1
-                    for (int c = 0; c < D / 16; ++c) {
-                        uint32_t ov[16];
-                        ld16(tmem_o + (uint32_t)(c * 16), ov);
-                        wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * alpha);
-                        st16(tmem_o + (uint32_t)(c * 16), ov);
+                        for (int e = 0; e < 16; ++e) {
+                            float x0, x1;
+                            unpair(fma2(pair_of(__uint_as_float(sv[c][2 * e]), __uint_as_float(sv[c][2 * e + 1])), factor2, off2), x0, x1);
+                            const float p0 = exp2_of(x0), p1 = exp2_of(x1);
+                            sum2[e & 3] = add2(sum2[e & 3], pair_of(p0, p1));
+                            const __half2 pk = __floats2half2_rn(p0, p1);
+                            pv[e] = *reinterpret_cast<const uint32_t*>(&pk);
+                        }
+                        st16(tmem_s + (uint32_t)(c * 16), pv);
                     }
-                    wait_st();
+                    float sum4[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { float x, z; unpair(sum2[i], x, z); sum4[i] = x + z; }
+                    row.l += (double)(((sum4[0] + sum4[1]) + (sum4[2] + sum4[3])) * exp2_of(-shift - P_SHIFT));
+                } else {
+                    row = one_by_one(f, tmem_s, tmem_o, row_factor, key0, row_lo, row_pos, b > 0, row);
                 }
-                const float off = (m_used == -INFINITY ? 0.f : shift - m_used) + P_SHIFT;
-                const uint64_t factor2 = pair_of(factor, factor), off2 = pair_of(off, off);
-                uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
-#pragma unroll
-                for (int c = 0; c < KEYS / 32; ++c) {
-                    uint32_t pv[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        float x0, x1;
-                        unpair(fma2(pair_of(__uint_as_float(sv[c][2 * e]), __uint_as_float(sv[c][2 * e + 1])), factor2, off2), x0, x1);
-                        const float p0 = exp2_of(x0), p1 = exp2_of(x1);
-                        sum2[e & 3] = add2(sum2[e & 3], pair_of(p0, p1));
-                        const __half2 pk = __floats2half2_rn(p0, p1);
-                        pv[e] = *reinterpret_cast<const uint32_t*>(&pk);
-                    }
-                    st16(tmem_s + (uint32_t)(c * 16), pv);
-                }
-                float sum4[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) { float x, z; unpair(sum2[i], x, z); sum4[i] = x + z; }
                 wait_st();
-                l = l * alpha + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3])) * exp2_of(-shift);
                 fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(sh.p_full + half);
@@ -472,7 +600,10 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
             alive = __all_sync(0xffffffffu, alive);
             if (alive) {
                 fence_after();
-                const float inverse = 1.f / l, unscale = exp2_of((float)base_exp);
+                const int l_exp = (__double2hiint(row.l) >> 20 & 0x7ff) - 1023;       // the sum is a number from 1 up to 2, times 2^l_exp
+                const bool none = row.l == 0.;
+                const Power unit = power_of((float)(base_exp - l_exp) - P_SHIFT);
+                const float inverse = unit.a / (float)(l_exp == 1024 ? row.l : __hiloint2double(__double2hiint(row.l) - (l_exp << 20), __double2loint(row.l)));
                 __nv_bfloat16* dst = out + ((size_t)(t.q_begin + t.tok0 + tok) * a.H + (size_t)kvh * G + head) * D;
 #pragma unroll 1
                 for (int c = 0; c < D / 16; ++c) {
@@ -485,8 +616,8 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                     __nv_bfloat162* op = reinterpret_cast<__nv_bfloat162*>(o4);
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        op[e] = l == 0.f ? __floats2bfloat162_rn(0.f, 0.f)
-                                         : __floats2bfloat162_rn(__uint_as_float(ov[2 * e]) * inverse * unscale, __uint_as_float(ov[2 * e + 1]) * inverse * unscale);
+                        op[e] = none ? __floats2bfloat162_rn(0.f, 0.f)
+                                     : __floats2bfloat162_rn(__uint_as_float(ov[2 * e]) * inverse * unit.b, __uint_as_float(ov[2 * e + 1]) * inverse * unit.b);
                     if (row_ok) {
                         reinterpret_cast<uint4*>(dst + 16 * c)[0] = o4[0];
                         reinterpret_cast<uint4*>(dst + 16 * c)[1] = o4[1];
@@ -498,10 +629,9 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                         if (!partial(key / KEYS - block0)) { key = key / KEYS * KEYS + KEYS - 1; continue; }
                         const int page = __ldg(table_row + a.page_of(key));
                         if (page < 0 || page >= a.num_pages) continue;
-                        const bool finite = fabsf(__ldg(a.v_scale + (size_t)page * a.KV + kvh)) < INFINITY;
                         const unsigned char* codes = a.v_cache + (long long)page * a.page_stride + a.row_in_page(key, kvh);
                         for (int d = 0; d < D; ++d)
-                            if (!finite || (__ldg(codes + d) & 0x7f) == 0x7f) dst[d] = __float2bfloat16_rn(__uint_as_float(0x7fffffffu));
+                            if ((__ldg(codes + d) & 0x7f) == 0x7f) dst[d] = __float2bfloat16_rn(__uint_as_float(0x7fffffffu));
                     }
                 }
             }

@@ -234,7 +234,9 @@ def paged_attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     ``window`` keys. A request may bring no token; a row that sees no key is zero; rows of ``out`` behind ``cu_q[-1]`` are left as they were.
     ``max_q_len``: no request brings more new tokens (one that does sets the status word and is left out); ``kv_len_bound``: about the longest context,
     which only decides how the keys are cut. No host list of tiles is needed, so the lengths may live on the GPU alone (see :func:`step_pages`).
-    Scores, sums and softmax are fp32; weights are rounded to 11 bits for bfloat16 queries, to 22 for float32 ones."""
+    Scores, sums and softmax are fp32; weights, times the value scale of their key, are rounded to 11 bits for bfloat16 queries, to 22 for float32 ones. Those of
+    less than 2^-17 of a row's largest (2^-29 in the kernel for few tokens) lose bits. Scales may be any numbers, zero, negative ones and NaN among them; those
+    that :func:`store_kv8` makes (powers of two) are the fast ones while the value scales of neighbouring pages lie within 2^4 of each other."""
     _here(q, "q")
     device = q.get_device()
     pages, page, kv, d, page_stride = _need_pools(device, k_cache, v_cache, k_scale, v_scale)
