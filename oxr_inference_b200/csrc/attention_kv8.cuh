@@ -107,22 +107,10 @@ struct Kv8Tile {
 };
 
 // The `index`-th tile over all requests, in their order: each warp of a block finds it for itself from the boundaries, so that neither host nor
-// an earlier kernel has to make a list. With one token a request at most, tile and request are one. `look`: this block also checks
-// that no request brings more than `any_q` tokens.
+// an earlier kernel has to make a list. `look`: this block also checks that no request brings more than `any_q` tokens.
 __device__ __forceinline__ Kv8Tile kv8_find_tile(const Kv8Args& a, int index, int tokens_per_tile, bool look) {
     Kv8Tile t = {-1, 0, 0, 0};
     const int lane = threadIdx.x & 31;
-    if (a.any_q == 1) {
-        if (index >= a.n) return t;
-        const int from = __ldg(a.cu_q + index), len = __ldg(a.cu_q + index + 1) - from;
-        if (len < 1) return t;
-        if (len > 1 || from < 0 || from >= a.n_tokens) {
-            if (threadIdx.x == 0) oxr_report(a.status, OXR_BAD_ARGUMENT, index);
-            return t;
-        }
-        t.req = index; t.q_begin = from; t.q_len = 1;
-        return t;
-    }
     int before = 0;
     for (int r0 = 0; r0 < a.n; r0 += 32) {
         const int r = r0 + lane;
