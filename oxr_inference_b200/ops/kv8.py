@@ -312,7 +312,9 @@ def step_pages(lengths: torch.Tensor, held: torch.Tensor, block_table: torch.Ten
     to come. Rows with ``fresh[r]`` other than 0 begin anew at length 0: their pages go on top of the stack ``free_list[:free_count[0]]``, row after row
     and page after page. Then every row takes the pages it lacks from the top, in the same order. A row that is given up is one with ``fresh`` 1 and
     ``q_lens`` 0. ``held``, ``block_table``, ``free_list`` and ``free_count`` are updated in place; with ``advance`` so is ``lengths`` (the step's tokens then count
-    as cached), without it the same step may be asked for again and takes nothing more.
+    as cached), without it ``lengths`` stays as it was, and a step of rows that go on may be asked for again: it takes nothing more and says the same. A row that
+    begins anew does so each time it is asked for: its pages go back and come again in another order. To ask for such a step again, set the row's length
+    and ``fresh`` to 0 first.
 
     All or nothing: if pages are lacking, a row does not fit its numbers (longer than ``width`` pages, a negative length) or the step brings more than
     ``tokens`` tokens, the status word is set, nothing moves, and the arrays hold no token at all (slots -1, ``cu_q`` and ``ctx_lens`` 0). The numbers of
