@@ -19,6 +19,8 @@ from oxr_inference_b200.parts.base import StepContext
 
 CHUNK = 64
 """Steps whose tokens are kept on the GPU before the host reads them."""
+LOOPS = 8
+"""Graphs that are kept: one for each number of requests and width of their tables, the ones used last."""
 
 
 @dataclass
@@ -64,9 +66,12 @@ class DeviceDecode:
         n, width = len(requests), 16
         while width < max(len(t) for rc in requests for t in rc.tables):
             width *= 2
-        loop = self._loops.get((n, width))
+        loop = self._loops.pop((n, width), None)
         if loop is None:
-            loop = self._loops[(n, width)] = self._capture(n, width)
+            while len(self._loops) >= LOOPS:      # (none is under way: each call waits for its own)
+                del self._loops[next(iter(self._loops))]
+            loop = self._capture(n, width)
+        self._loops[(n, width)] = loop      # the last to go
 
         def put(dst: torch.Tensor, values: list) -> None:
             dst.copy_(torch.tensor(values, dtype=dst.dtype).view(dst.shape))
