@@ -49,12 +49,16 @@ class DeviceDecode:
     @torch.inference_mode()
     def run(self, requests: list[RequestCache], tokens: list[int], steps: int) -> list[list[int]]:
         """The next ``steps`` tokens of each request, greedily (the first largest logit), from ``tokens``: the last token each has, not yet in its cache.
-        Afterwards each request's cache holds ``steps`` tokens more: the given one and all but the last of those returned."""
+        Afterwards each request's cache holds ``steps`` tokens more: the given one and all but the last of those returned. If a kernel reports an error
+        (RuntimeError), the requests' lengths are as before, but their pages and states are not: they have to be closed."""
         m = self.runner.cache
         if not requests or len(requests) != len(tokens) or steps < 1:
             raise ValueError(f"{len(requests)} requests, {len(tokens)} tokens, {steps} steps")
         if len({id(rc) for rc in requests}) != len(requests):
             raise ValueError("a request is given twice")
+        vocabulary = self.runner.model.spec.vocab_size
+        if not all(0 <= t < vocabulary for t in tokens):
+            raise ValueError(f"a token outside the vocabulary of {vocabulary}")
         if not m.pools:
             raise ValueError("the model keeps no pages; its steps need no tables")
         longest = max(rc.length for rc in requests) + steps

@@ -30,3 +30,19 @@ def test_only_the_last_graphs_are_kept(folders, monkeypatch):  # noqa: F811
     assert kept == [[3], [3, 2], [2, 3], [3, 1], [1, 2], [2, 3], [2, 3]]
     monkeypatch.setattr(device_decode, "LOOPS", 8)
     assert decoded((3, 2, 3, 1, 2, 3, 3))[0] == out
+
+
+def test_tokens_outside_the_vocabulary_are_refused_before_anything_moves(tmp_path):
+    """Recurrent states cannot be taken back once a step has run."""
+    import radapel_util
+
+    folder = radapel_util.make_folder(tmp_path, radapel_util.MODEL_X, "x", 3)
+    r, s = (make(folder, "radapel", "float32", page=8) for _ in range(2))
+    prompts = [[5, 17, 3, 9], [9, 8, 7]]
+    (caches, tokens), (caches2, tokens2) = begin(r, prompts), begin(s, prompts)
+    free = s.cache.free_pages
+    for bad in (-1, s.model.spec.vocab_size, 1 << 40):
+        with pytest.raises(ValueError, match="vocabulary"):
+            s.decode(caches2, [tokens2[0], bad], 4)
+    assert s.cache.free_pages == free and [rc.length for rc in caches2] == [4, 3]
+    assert s.decode(caches2, tokens2, 4) == r.decode(caches, tokens, 4)
