@@ -47,6 +47,8 @@ class EngineSettings:
             raise ValueError(f"dtype must be 'bfloat16' or 'float32', got {self.dtype!r}")
         if self.kv_cache_dtype not in ("auto", "e4m3"):
             raise ValueError(f"kv_cache_dtype must be 'auto' or 'e4m3', got {self.kv_cache_dtype!r}")
+        if self.kv_cache_dtype == "e4m3" and self.page_size > 8192:
+            raise ValueError(f"page_size {self.page_size}: pages of 8-bit keys and values hold up to 8192 tokens")
         if self.page_size <= 0:
             raise ValueError("page_size must be positive")
         if self.max_step_tokens < 1 or self.prefill_chunk < 1 or self.max_running < 1:

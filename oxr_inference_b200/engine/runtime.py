@@ -60,6 +60,8 @@ class ModelRunner:
         spec = arch.spec_for(config, shapes)
         runtime = Runtime(device=dev, dtype=DTYPES[dtype], max_positions=max_positions or spec.max_positions,
                           status=ops.new_status(dev), page_size=page_size, kv_dtype=kv_cache_dtype)
+        if kv_cache_dtype == "e4m3" and page_size > ops.KV8_LONGEST_PAGE:
+            raise ValueError(f"page_size {page_size}: pages of 8-bit keys and values hold up to {ops.KV8_LONGEST_PAGE} tokens")
         model = DecoderModel(spec, runtime)
         if kv_cache_dtype != "auto" and not any(g.need.eight_bit for g in model.cache_plan.groups):
             raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r}: no layer of this model keeps keys and values that could be held in 8 bits")

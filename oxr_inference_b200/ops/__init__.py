@@ -2455,4 +2455,4 @@ def diff_combine(o: torch.Tensor, num_heads: int, value_dim: int, lam: torch.Ten
     return out
 
 
-from oxr_inference_b200.ops.kv8 import KV8_DTYPE, PageStep, paged_attention_kv8, step_pages, store_kv8, warm_up_kv8  # noqa: E402, F401
+from oxr_inference_b200.ops.kv8 import KV8_DTYPE, KV8_LONGEST_PAGE, PageStep, paged_attention_kv8, step_pages, store_kv8, warm_up_kv8  # noqa: E402, F401

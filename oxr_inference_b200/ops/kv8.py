@@ -22,6 +22,8 @@ from oxr_inference_b200.ops.build import BuildError
 KV8_DTYPE = torch.float8_e4m3fn
 KV8_FEW_TOKENS = 1024
 """Up to so many tokens the store looks through all slots itself; for more it takes scratch of two words a page."""
+KV8_LONGEST_PAGE = 8192
+"""Tokens of a page that the store takes at most."""
 _INT, _F32 = torch.int32, torch.float32
 
 # The calls' arguments, each in one block as the libraries declare it: pointers first, then 64-bit and 32-bit numbers.
@@ -153,8 +155,8 @@ def store_kv8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: to
     if slots.dim() != 1 or k.shape != (n, kv, d) or v.shape != (n, kv, d) or k.dtype != v.dtype:
         raise ops.KernelError(f"k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} must be [{n}, {kv}, {d}] of one dtype for {n} slots")
     code = ops._dtype_code(k)
-    if page > 8192 or pages * page > 0x80000000 - 8192:
-        raise ops.KernelError(f"{pages} pages of {page} tokens: the store takes pages of up to 8192, slots below 2^31 - 8192")
+    if page > KV8_LONGEST_PAGE or pages * page > 0x80000000 - KV8_LONGEST_PAGE:
+        raise ops.KernelError(f"{pages} pages of {page} tokens: the store takes pages of up to {KV8_LONGEST_PAGE}, slots below 2^31 - {KV8_LONGEST_PAGE}")
     k_stride, v_stride = _head_rows(k, "k", device), _head_rows(v, "v", device)
     if n == 0:
         return
