@@ -647,6 +647,16 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
 }  // namespace
 #endif
 
+// Whether the kernel may run at all. setmaxnreg deals out what the block is launched with: 128 registers a thread, or the softmax warps would wait for
+// theirs in vain.
+OXR_API int oxr_kv8_prompt_ready() {
+#if HEAD_DIM <= 128
+    cudaFuncAttributes attrs;
+    if (cudaFuncGetAttributes(&attrs, attn_kv8_prompt_kernel) == cudaSuccess) return attrs.numRegs == 128;
+    cudaGetLastError();
+#endif
+    return 0;
+}
 // For bf16 queries, head sizes up to 128 and a positive scale.
 OXR_API int oxr_kv8_prompt_attention(const Kv8Call* c) {
 #if HEAD_DIM <= 128
@@ -659,10 +669,7 @@ OXR_API int oxr_kv8_prompt_attention(const Kv8Call* c) {
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess) return oxr_launch_status();
     if (ready != device) {
-        // setmaxnreg deals out what the block is launched with: 128 registers a thread, or the softmax warps would wait for theirs in vain
-        cudaFuncAttributes attrs;
-        if (cudaFuncGetAttributes(&attrs, attn_kv8_prompt_kernel) != cudaSuccess) return oxr_launch_status();
-        if (attrs.numRegs != 128) return OXR_BAD_ARGUMENT;
+        if (!oxr_kv8_prompt_ready()) return OXR_BAD_ARGUMENT;
         if (cudaFuncSetAttribute(attn_kv8_prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM) != cudaSuccess) return oxr_launch_status();
         ready = device;
     }

@@ -43,6 +43,7 @@ def _kv8_lib(head_dim: int):
         lib.oxr_kv8_attention.restype = c_int
         lib.oxr_kv8_prompt_attention.argtypes = [c_char_p]
         lib.oxr_kv8_prompt_attention.restype = c_int
+        lib.oxr_kv8_prompt_ready.restype = c_int
         lib.oxr_kv8_blocks_per_sm.argtypes = [c_int, c_int]
         lib.oxr_kv8_blocks_per_sm.restype = c_int
         lib.oxr_kv8_head_dim.restype = c_int
@@ -196,6 +197,12 @@ KV8_PROMPT_ROWS = 256
 """Rows of a tile of the tcgen05 kernel for long portions."""
 
 
+@functools.lru_cache(maxsize=None)
+def kv8_prompt_runs(head_dim: int) -> bool:
+    """Whether this build of the tcgen05 kernel can run: its split of the registers is for 128 a thread, which is the compiler's choice."""
+    return bool(_kv8_lib(head_dim).oxr_kv8_prompt_ready())
+
+
 def kv8_prompt_takes(max_q_len: int, head_dim: int, dtype: torch.dtype, scale: float) -> bool:
     """Whether the tcgen05 kernel can take the longer portions of a step: bfloat16 queries, head sizes up to 128, a positive scale (it scales a row's maximum,
     not each score)."""
@@ -273,7 +280,7 @@ def paged_attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
                 block_table.data_ptr())
     sizes = (page_stride, q_stride, n, tokens, block_table.shape[1], page, pages, heads, kv, window)
     seen = max(1, min(kv_len_bound, window + max_q_len) if window > 0 else kv_len_bound)
-    if max_q_len > ops.SHORT_MAX_TOKENS and kv8_prompt_takes(max_q_len, d, q.dtype, scale) and kv8_prompt_pays(n, tokens, max_q_len, heads, kv, d, seen):
+    if max_q_len > ops.SHORT_MAX_TOKENS and kv8_prompt_takes(max_q_len, d, q.dtype, scale) and kv8_prompt_pays(n, tokens, max_q_len, heads, kv, d, seen) and kv8_prompt_runs(d):
         fewest = ops.SHORT_MAX_TOKENS + 1 if n > 1 else 1      # a request alone goes there whatever it brings
         tiles = min(tokens, min(n, tokens // fewest) + tokens // (KV8_PROMPT_ROWS // min(group, KV8_PROMPT_ROWS)))
         call = _ATTENTION_CALL(*pointers, 0, status.data_ptr(), stream, *sizes, fewest, max_q_len, max_q_len, 0, tiles, code, scale)

@@ -118,3 +118,14 @@ def test_rows_differ_in_what_they_see(status, seed):  # noqa: F811
         got = b.run(status).double().cpu()[:at]
         fine(status)
         assert bool(((got - want[:at]).abs() <= tol).all())
+
+
+def test_a_build_that_cannot_run_the_kernel_leaves_its_steps_to_the_other(status, monkeypatch):  # noqa: F811
+    b = S.sizes(CASES[1], seed=1)
+    monkeypatch.setattr(kv8, "kv8_prompt_runs", lambda d: False)
+    b.check(status)
+    got = b.run(status)
+    monkeypatch.setattr(kv8, "kv8_prompt_pays", lambda *a: False)
+    assert torch.equal(b.run(status), got)
+    monkeypatch.undo()
+    assert kv8.kv8_prompt_runs(128) and kv8.kv8_prompt_runs(16) and not kv8.kv8_prompt_runs(144)
