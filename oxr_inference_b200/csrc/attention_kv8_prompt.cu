@@ -25,7 +25,7 @@
 // Every wait on an mbarrier is bounded.
 #include <cuda_fp16.h>
 
-#include "tma.cuh"
+#include "umma.cuh"
 
 #ifndef HEAD_DIM
 #error "compile with -DHEAD_DIM=<head size>"
@@ -70,27 +70,17 @@ struct Shared {
 constexpr size_t SMEM = (2 + 2 * STAGES) * (size_t)TENSOR_BYTES + sizeof(Shared);
 static_assert(SMEM <= 227 * 1024, "shared memory of a block");
 
-__device__ __forceinline__ uint64_t desc_kmajor(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
 // rows are keys (the products' depth), 64 entries in 128 bytes; the next 64 entries a panel on
 __device__ __forceinline__ uint64_t desc_mnmajor(uint32_t saddr) {
     return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(PANEL_BYTES >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-// kind::f16, fp32 sums, both operands fp16, A K-major, B K-major or MN-major
+// kind::f16, fp32 sums, both operands fp16, A K-major, B K-major or MN-major (the product itself is the one that umma_bf16 issues: the descriptor has the types)
 __host__ __device__ constexpr uint32_t idesc_of(int m, int n, bool b_mn_major) {
     return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
-                 ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
 }
 __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
                  ::"r"(d), "r"(ta), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
-}
-__device__ __forceinline__ void commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 #define KV8_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define KV8_I8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
@@ -112,11 +102,6 @@ __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ bool one_lane() {
-    uint32_t pred;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
-    return pred != 0;
-}
 // Two fp32 numbers in a pair of registers, for the packed fp32 instructions.
 __device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
     uint64_t r;
@@ -452,7 +437,7 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                 loaders_meet();
             }
             if (!ok && lane == 0) oxr_report(a.status, OXR_WAIT_EXPIRED, 41);
-        } else if (one_lane()) {
+        } else if (elect_one()) {
             // ------------------------------------------------------------------ the products
             constexpr uint32_t idesc_s = idesc_of(HALF_ROWS, KEYS, false), idesc_o = idesc_of(HALF_ROWS, O_COLS, true);
             const int halves = half1_live ? 2 : 1;
@@ -466,10 +451,10 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                 const uint32_t ka = smem_addr(k_ring + (b % STAGES) * TENSOR_BYTES), qa = smem_addr(q_tiles + h * TENSOR_BYTES);
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk)
-                    mma_smem(tmem + (uint32_t)(h * KEYS), desc_kmajor(qa + (kk >> 2) * PANEL_BYTES + (kk & 3) * 32), desc_kmajor(ka + (kk >> 2) * PANEL_BYTES + (kk & 3) * 32),
+                    umma_bf16(tmem + (uint32_t)(h * KEYS), umma_desc(qa + (kk >> 2) * PANEL_BYTES + (kk & 3) * 32), umma_desc(ka + (kk >> 2) * PANEL_BYTES + (kk & 3) * 32),
                              idesc_s, kk > 0 ? 1u : 0u);
-                commit(sh.s_full + h);
-                if (h == halves - 1) commit(sh.k_empty + b % STAGES);
+                umma_commit(sh.s_full + h);
+                if (h == halves - 1) umma_commit(sh.k_empty + b % STAGES);
             };
             ok = ok && wait_for(&sh.q_ready, 0, 42) && wait_for(sh.k_full, 0, 43);
             if (ok)
@@ -483,8 +468,8 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
 #pragma unroll
                     for (int kk = 0; kk < KEYS / 16; ++kk)
                         mma_tmem(tmem + 256 + (uint32_t)(h * O_COLS), tmem + (uint32_t)(h * KEYS + kk * 8), desc_mnmajor(va + kk * 16 * 128), idesc_o, (b > 0 || kk > 0) ? 1u : 0u);
-                    commit(sh.o_done + h);
-                    if (h == halves - 1) commit(sh.v_empty + b % STAGES);
+                    umma_commit(sh.o_done + h);
+                    if (h == halves - 1) umma_commit(sh.v_empty + b % STAGES);
                     if (b + 1 < count) {
                         ok = h > 0 || wait_for(sh.k_full + (b + 1) % STAGES, ((b + 1) / STAGES) & 1, 43);
                         if (ok) issue_s(b + 1, h);
