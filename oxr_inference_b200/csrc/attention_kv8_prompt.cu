@@ -414,6 +414,7 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
             }
             ask(kc, a.k_cache, 0);
             ask(vc, a.v_cache, 0);
+            loaders_meet();        // the first block's rows have been read: an uneven one's exponents come over them
             bool ok = true;        // (a thread that has given up keeps meeting the others)
             for (int b = 0; b < count; ++b) {
                 BlockInfo& f = sh.info[b % INFO];
