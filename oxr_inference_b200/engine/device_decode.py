@@ -15,6 +15,7 @@ import torch
 
 from oxr_inference_b200 import ops
 from oxr_inference_b200.cache.manager import RequestCache, pages_for
+from oxr_inference_b200.engine.runtime import no_collection
 from oxr_inference_b200.parts.base import StepContext
 
 CHUNK = 64
@@ -142,7 +143,7 @@ class DeviceDecode:
             self._pool = torch.cuda.graph_pool_handle()
         before = ops.launch_count
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.stream(side):
+        with torch.cuda.stream(side), no_collection():
             graph.capture_begin(pool=self._pool)
             try:
                 self._step(n, width, loop)

@@ -16,7 +16,7 @@ import torch
 
 from oxr_inference_b200 import ops
 from oxr_inference_b200.engine.batch import Layout, StepEntry
-from oxr_inference_b200.engine.runtime import ModelRunner
+from oxr_inference_b200.engine.runtime import ModelRunner, no_collection
 from oxr_inference_b200.parts.base import uneven_lengths
 
 BUCKETS = (1, 2, 4, 8, 16, 32, 64, 128, 192, 256, 384, 512, 768, 1024)  # oxr_runtime/decode_graph.py:30
@@ -96,9 +96,9 @@ class DecodeGraphs:
         status = self.runner.model.runtime.status
         # capture_begin / capture_end directly: the `torch.cuda.graph` context also collects garbage and empties the
         # allocator's cache first, which costs a serving engine 0.2 to 0.7 s per new bucket (the capture itself and then
-        # every buffer of the next mixed step allocated afresh)
+        # every buffer of the next mixed step allocated afresh); garbage is left for later instead
         side.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(side):
+        with torch.cuda.stream(side), no_collection():
             graph.capture_begin(pool=self._pool)
             try:
                 block.copy_(staging, non_blocking=True)

@@ -2,8 +2,10 @@
 
 from __future__ import annotations
 
+import gc
+from contextlib import contextmanager
 from pathlib import Path
-from typing import Any, Mapping
+from typing import Any, Iterator, Mapping
 
 import torch
 
@@ -31,6 +33,18 @@ def require_cuda(device: str | torch.device = "cuda") -> torch.device:
     torch.backends.cuda.matmul.allow_tf32 = False
     torch.backends.cuda.matmul.allow_bf16_reduced_precision_reduction = False
     return device
+
+
+@contextmanager
+def no_collection() -> Iterator[None]:
+    """Garbage stays where it is while a CUDA graph is captured: what it frees on the GPU (another graph, in the first place) would make the capture invalid."""
+    was = gc.isenabled()
+    gc.disable()
+    try:
+        yield
+    finally:
+        if was:
+            gc.enable()
 
 
 class ModelRunner:
