@@ -9,6 +9,7 @@ graph once per step and reads the tokens at the end.
 
 from __future__ import annotations
 
+import weakref
 from dataclasses import dataclass
 
 import torch
@@ -43,7 +44,7 @@ class _Loop:
 
 class DeviceDecode:
     def __init__(self, runner):
-        self.runner = runner
+        self.runner = weakref.proxy(runner)      # (which owns this: a circle would keep graphs and pools until garbage is collected)
         self._loops: dict[tuple[int, int], _Loop] = {}
         self._pool = None
 

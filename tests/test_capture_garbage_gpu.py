@@ -1,6 +1,7 @@
 """Captures of decode steps while there is garbage that holds CUDA graphs, and what keeps graphs alive."""
 
 import gc
+import weakref
 
 import pytest
 import torch
@@ -72,3 +73,18 @@ def test_captures_of_an_engine(folders):  # noqa: F811
     with_garbage(made.runner.model, stock)
     assert [c.token_ids for c in made.generate(prompts, params)] == want
     assert made.counters["graph_steps"] > 0 and gc.isenabled()
+
+
+def test_a_runner_goes_with_its_last_name(folders):  # noqa: F811
+    """Its graphs, weights and pools do not wait for the collector."""
+    r = make(folders["A"], "A", "float32")
+    caches, tokens = begin(r, [util.token_ids("A", 9, seed=3)])
+    assert len(r.decode(caches, tokens, 3)[0]) == 3
+    gone = weakref.ref(r)
+    gc.collect()
+    gc.disable()
+    try:
+        del r
+        assert gone() is None
+    finally:
+        gc.enable()
