@@ -28,7 +28,7 @@
 // grid takes an equal stretch of it, so that requests of any lengths keep all of them busy to the end; the boundaries are worked out on the GPU, from
 // the lengths. A warp is on its own: a ring of stages filled by TMA (with cp.async where pages are not multiples of eight keys), one online softmax,
 // no barrier. What it has of a tile that it does not have whole goes to scratch memory, and a second kernel joins those pieces. What bounds it
-// is reading the cache: 2 D bytes per key and KV head. 64 requests of 2,048 keys, 32 / 8 heads of 128: 54 us (5.0 TB/s, 0.76 of measured) and 5 for
+// is reading the cache: 2 D bytes per key and KV head. 64 requests of 2,048 keys, 32 / 8 heads of 128: 55 us (4.9 TB/s, 0.75 of measured) and 6 for
 // the join; the rest is the latency of a warp's chain of conversions, products and softmax at the twelve warps that an SM's registers hold.
 #include <cuda_fp16.h>
 #include <type_traits>
