@@ -20,7 +20,7 @@
 // much the scales of pages differ and whatever scales pages have that the row does not see or gives no weight. The sum of the weights without their
 // scales may lie as far from m as scales reach, 2^+-250.
 // The ordinary walk over a tile's blocks takes one power for the value scales of a block, so that the sum follows from the weighted weights, and a float for the
-// sum. That is good while the scales of a block lie within 2^4 of each other, and all of them within 2^30 of the last page's, which is their unit (and not below 2^-110). A warp that
+// sum. That is good while the scales of a block lie within 2^4 of each other, and all of them within 2^30 of the last page's, which is their unit (and not below 2^-110); blocks of zeros alone count as of 2^-60. A warp that
 // meets others begins its part of the tile anew in a careful walk, where the sum has a power of two beside it and a block is gone through once for each 2^4 that its
 // scales span. (One walk for both issued 14 % more instructions: 64 requests of 2,048 keys 64 us instead of 61.)
 //
@@ -559,10 +559,10 @@ attn_kv8_kernel(T* __restrict__ out, const T* __restrict__ q, const __grid_const
         }
         // 2^lv: the power above the largest value scale, relative to the last page's scale; `now`: the keys whose scales lie within 2^4 of it
         const bool finite = most_vs < 0x7f800000u;
-        const int most_exp = finite ? scale_exponent(__uint_as_float(most_vs)) : base_exp, lv = most_vs ? most_exp - base_exp : NO_SCALE;
+        const int most_exp = !finite ? base_exp : most_vs ? scale_exponent(__uint_as_float(most_vs)) : 0, lv = most_vs ? most_exp - base_exp : CAREFUL ? NO_SCALE : -60;
         uint32_t now = left_keys;
         if constexpr (!CAREFUL) {
-            if (!finite || least_vs == 0u || most_vs - least_vs > 4u << 23 || lv > 30 || lv < -30 || most_exp < -110) {
+            if (!finite || (most_vs && (least_vs == 0u || most_vs - least_vs > 4u << 23 || lv > 30 || lv < -30 || most_exp < -110))) {
                 const bool all = arrived(i + 1, i + STAGES);
                 if (!all && lane == 0) oxr_report(a.status, OXR_WAIT_EXPIRED, 40);
                 fence_proxy_async();

@@ -374,10 +374,10 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                 BlockInfo& f = sh.info[b % INFO];
                 const float km = most_of(f.k_most), vm = most_of(f.v_most);
                 const float kr = __fdividef(ks, km), vr = __fdividef(vs, vm);
-                const bool k_exact = exact(kr, K_LEAST) || ks == 0.f, v_exact = exact(vr, V_LEAST);
+                const bool k_exact = exact(kr, K_LEAST) || ks == 0.f, v_none = vm == 0.f && vs == 0.f, v_exact = exact(vr, V_LEAST) || v_none;
                 f.k_ratio[lt] = __float2half2_rn(k_exact ? (ks == 0.f ? 0.f : kr) : 1.f);
-                f.v_ratio[lt] = __float2half2_rn(v_exact ? vr : 1.f);
-                const float shift = fmaxf(log2f(vm) - (float)base_exp, (float)NO_SCALE);
+                f.v_ratio[lt] = __float2half2_rn(v_exact ? (v_none ? 0.f : vr) : 1.f);
+                const float shift = vm > 0.f ? log2f(vm) - (float)base_exp : -60.f;      // (values of zero alone count as of 2^-60)
                 top = fmaxf(top, shift);
                 if (page >= 0 && !(k_exact && v_exact && fabsf(shift) <= 60.f && shift >= top - 60.f)) f.even = 0;
                 if (lt == 0) {

@@ -129,3 +129,10 @@ def test_a_build_that_cannot_run_the_kernel_leaves_its_steps_to_the_other(status
     assert torch.equal(b.run(status), got)
     monkeypatch.undo()
     assert kv8.kv8_prompt_runs(128) and kv8.kv8_prompt_runs(16) and not kv8.kv8_prompt_runs(144)
+
+
+@by_size
+@pytest.mark.parametrize("lean", [0, 30, 50, 70, -20])
+@pytest.mark.parametrize("zeros", ["first", "last", "all"])
+def test_blocks_of_zeros(status, case, lean, zeros):  # noqa: F811
+    S.test_blocks_of_zeros(status, case, lean, zeros)

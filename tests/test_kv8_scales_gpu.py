@@ -201,3 +201,19 @@ def test_one_page_among_many_makes_its_warp_begin_anew(status):  # noqa: F811
             b.check(status)
             want = b.run(status)
             assert all(torch.equal(b.run(status), want) for _ in range(5))
+
+
+@pytest.mark.parametrize("case", SPLIT, ids=name_of)
+@pytest.mark.parametrize("lean", [0, 30, 50, 70, -20])
+@pytest.mark.parametrize("zeros", ["first", "last", "all"])
+def test_blocks_of_zeros(status, case, lean, zeros):  # noqa: F811
+    """Half of a context, or all of it, holds nothing but zeros, with scales of 0: its keys have their weights all the same."""
+    b = leaning(case, lean)
+    e = torch.full(tuple(b.vs.shape), -6.0)
+    b.vs = powers(e)
+    for t, ctx in zip(b.tables, b.ctx_lens):
+        cut = -(-ctx // b.page // 2)
+        b.vs[t if zeros == "all" else t[:cut] if zeros == "first" else t[cut:]] = 0
+    b.check(status)
+    if zeros == "all":
+        assert bool((b.run(status) == 0).all())
