@@ -8,22 +8,27 @@
 // kind::f8f6f4 would take the codes as they are, but its other operand would have to have 8 bits too, and two e4m3 numbers for each weight cost the
 // softmax threads more than what is done instead: seven warps turn the codes of a block, while it passes from global to shared memory, into fp16
 // numbers, times the ratio of their scale to the block's largest where that is a power of two and the products are exact: for keys from 2^-14 on, for values
-// from 2^-4 on, which leaves the weights their bits; elsewhere times 1. In an even block that is so of all keys (and the largest value scale within 2^60 of the last
-// page's), as it mostly is among the store's scales: the largest key scale goes into the factor of the scores, the largest value scale, as its logarithm, into the exponent of
-// the weights, and neither costs the softmax an instruction per key. In other blocks (and in one whose value scales are 2^60 below some met before) the softmax
-// takes keys one by one, each with its own scales. As in the split-key kernel the maximum is that of score and value scale, in whole numbers, and the sum of
-// the weights a double: a row's result does not hang on scales that it does not see or gives no weight.
+// from 2^-4 on, which leaves the weights their bits; elsewhere times 1. There are three kinds of blocks:
+//     EVEN   all ratios are such, as mostly among the store's scales: the largest key scale goes into the factor of the scores, the largest value scale, as its
+//            logarithm, into the exponent of the weights, and neither costs the softmax an instruction per key;
+//     NEAR   the value scales lie within 2^4 of the largest all the same (and key scales below 2^64): scores and weights are multiplied by what is left of their
+//            keys' scales, in fp32;
+//     ODD    any others, and blocks whose value scales are 2^60 off the last page's or below some met before: keys one by one, with two exponentials each.
+// As in the split-key kernel the maximum is that of score and value scale, in whole numbers, and the sum of the weights a double: a row's result does not hang on
+// scales that it does not see or gives no weight.
 // Weights are kept as 2^7 P against a maximum that is raised in steps of 2^8: below 2^15 in
-// fp16, with their eleven bits down to 2^-21 of the largest (2^-17 in an even block).
+// fp16, with their eleven bits down to 2^-21 of the largest (2^-17 where one power stands for a block's scales).
 // Warps: 0 issues the products and owns the tensor memory, 1 to 3 and 12 to 15 bring in keys and values, 4 to 7 and 8 to 11 are the
 // softmax of the first and the second half; setmaxnreg gives those 160 registers (128 scores and what goes with them) and the others 96 (with 64 the
 // codes on their way were spilled: 404 us instead of 146 in the case below).
 // What bounds it: per block of 128 keys the products take 2,048 cycles of the tensor pipe and about as much shared-memory bandwidth, the exponentials 2,048 of
-// theirs. 2,048 tokens on 2,048 cached ones, 32 / 8 heads of 128, take 146 us (706 TFLOP/s, 0.43 of measured): 2.9 us a block. Without the loaders' work it would be 120,
-// without the softmax's arithmetic 133: two chains of latencies that are equally long and share the issue slots. With scales of any mantissa, every block of them
-// uneven, it takes 320.
+// theirs. 2,048 tokens on 2,048 cached ones, 32 / 8 heads of 128, take 148 us (697 TFLOP/s, 0.42 of measured): 2.9 us a block. Without the loaders' work it would be 120,
+// without the softmax's arithmetic 133: two chains of latencies that are equally long and share the issue slots. With all blocks NEAR, scales of any mantissa, it takes 170, with
+// all ODD 325. (NEAR and EVEN in one piece of code: 165 for EVEN blocks, whose registers were spilled.)
 // Every wait on an mbarrier is bounded.
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "umma.cuh"
 
@@ -44,6 +49,7 @@ constexpr int O_COLS = PANELS * 64;                      // whole panels: what t
 constexpr int WORDS = D / 16;                            // 16 codes of a key: what a loader thread takes at a time
 constexpr int PASSES = (KEYS * WORDS + LOADERS - 1) / LOADERS;
 constexpr int INFO = 4;                                  // blocks whose pages and scales are at hand
+constexpr int ODD = 0, NEAR = 1, EVEN = 2;
 constexpr float RAISE = 8.f;
 constexpr float P_SHIFT = 7.f;
 constexpr uint32_t TMEM_COLS = 512;                      // S | P of half h at 128 h, O of half h at 256 + h O_COLS
@@ -51,14 +57,14 @@ constexpr uint32_t TMEM_COLS = 512;                      // S | P of half h at 1
 struct __align__(16) BlockInfo {
     union {
         long long row[KEYS];   // byte offset of each key's row in the pools; -1: zeros stand for it
-        float v_exp[KEYS];     // of an uneven block, once its codes have been asked for
+        float v_exp[KEYS];     // of an ODD block, once its codes have been asked for
     };
-    // Scales; of an uneven block then what is left of them beside the ratios: a factor of a key's scores, and of its values a power of two, as its exponent
-    // relative to the last page's, and a factor of up to 1.
+    // Scales; of blocks that are not EVEN then what is left of them beside the ratios: a factor of a key's scores, and of its values a factor of up to 1 and in an ODD
+    // block a power of two, as its exponent relative to the last page's.
     float k_scale[KEYS], v_scale[KEYS];
     __half2 k_ratio[KEYS], v_ratio[KEYS];   // what codes are multiplied by: a scale over the block's largest, or 1 where that is not exact
     float k_most[4], v_most[4];   // of each 32 keys: the largest scale
-    int even;                  // all of them are exact
+    int kind;                  // EVEN: all of them are exact; NEAR: the value scales lie within 2^4 of the largest all the same; else ODD
     float factor, shift;       // of the block: its largest key scale; log2 of its largest value scale, relative to the last page's
 };
 struct Shared {
@@ -119,6 +125,14 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+// Four numbers by four others.
+__device__ __forceinline__ void by_four(uint32_t* x, const float4& k) {
+    float z[4];
+    unpair(fma2(pair_of(__uint_as_float(x[0]), __uint_as_float(x[1])), pair_of(k.x, k.y), 0ull), z[0], z[1]);
+    unpair(fma2(pair_of(__uint_as_float(x[2]), __uint_as_float(x[3])), pair_of(k.z, k.w), 0ull), z[2], z[3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __float_as_uint(z[i]);
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -160,7 +174,7 @@ __device__ __forceinline__ void raise_row(Row& row, float mx, uint32_t tmem_o, b
         wait_st();
     }
 }
-// The softmax of an uneven block, key by key; a row sees keys row_lo .. row_pos. By whole warps. (A function of its own: inlined it took registers from the ordinary
+// The softmax of an ODD block, key by key; a row sees keys row_lo .. row_pos. By whole warps. (A function of its own: inlined it took registers from the ordinary
 // block's softmax.)
 __device__ __noinline__ Row one_by_one(const BlockInfo& f, uint32_t tmem_s, uint32_t tmem_o, float row_factor, int key0, int row_lo, int row_pos, bool begun, Row row) {
     // The scores of 32 keys, the hidden ones' -inf.
@@ -294,7 +308,7 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                 f.k_scale[lt] = ks;
                 f.v_scale[lt] = vs;
                 f.row[lt] = page >= 0 ? (long long)page * a.page_stride + a.row_in_page(key, kvh) : -1;
-                if (lt == 0) f.even = 1;
+                if (lt == 0) f.kind = EVEN;
                 // (positive floats compare as integers do)
                 const uint32_t km = __reduce_max_sync(0xffffffffu, __float_as_uint(usable(ks))), vm = __reduce_max_sync(0xffffffffu, __float_as_uint(usable(vs)));
                 if (lane == 0) { f.k_most[lt / 32] = __uint_as_float(km); f.v_most[lt / 32] = __uint_as_float(vm); }
@@ -379,19 +393,26 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                 f.v_ratio[lt] = __float2half2_rn(v_exact ? (v_none ? 0.f : vr) : 1.f);
                 const float shift = vm > 0.f ? log2f(vm) - (float)base_exp : -60.f;      // (values of zero alone count as of 2^-60)
                 top = fmaxf(top, shift);
-                if (page >= 0 && !(k_exact && v_exact && fabsf(shift) <= 60.f && shift >= top - 60.f)) f.even = 0;
+                if (page >= 0) {
+                    const bool near = v_none || (vr >= 0.0625f && vr <= 1.00001f);
+                    const bool fits = k_exact || !(fabsf(ks) > 1.8e19f);      // 2^64: a score times it stays a float
+                    if (!(near && fits && fabsf(shift) <= 60.f && shift >= top - 60.f)) atomicMin(&f.kind, ODD);
+                    else if (!k_exact || !v_exact) atomicMin(&f.kind, NEAR);
+                }
                 if (lt == 0) {
                     f.factor = km > 0.f ? km : 1.f;
                     f.shift = shift;
                 }
             };
-            // What the softmax needs for the keys of an uneven block.
+            // What the softmax needs for the keys of a block that is not EVEN.
             auto put_parts = [&](BlockInfo& f) {
                 const float km = most_of(f.k_most), vm = most_of(f.v_most), ks = f.k_scale[lt], vs = f.v_scale[lt];
                 if (exact(__fdividef(ks, km), K_LEAST)) f.k_scale[lt] = km;
                 if (exact(__fdividef(vs, vm), V_LEAST)) {
                     f.v_exp[lt] = f.shift;
                     f.v_scale[lt] = 1.f;
+                } else if (f.kind == NEAR) {
+                    f.v_scale[lt] = vm > 0.f ? __fdividef(vs, vm) : 0.f;
                 } else {
                     const int up = fabsf(vs) < INFINITY ? scale_exponent(fabsf(vs)) : base_exp;
                     const Power unit = power_of(-(float)up);
@@ -414,14 +435,14 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
             }
             ask(kc, a.k_cache, 0);
             ask(vc, a.v_cache, 0);
-            loaders_meet();        // the first block's rows have been read: an uneven one's exponents come over them
+            loaders_meet();        // the first block's rows have been read: an ODD one's exponents come over them
             bool ok = true;        // (a thread that has given up keeps meeting the others)
             for (int b = 0; b < count; ++b) {
                 BlockInfo& f = sh.info[b % INFO];
                 const int st = b % STAGES;
                 const float ks = scale_of(a.k_scale, page2), vs = scale_of(a.v_scale, page2);      // of block b + 2
                 const int page3 = page_for(b + 3);
-                if (lt < KEYS && !f.even) put_parts(f);      // (its rows have been asked for)
+                if (lt < KEYS && f.kind != EVEN) put_parts(f);      // (its rows have been asked for)
                 ok = ok && mbar_wait(sh.k_empty + st, ((b / STAGES) & 1) ^ 1);
                 put(kc, k_ring + st * TENSOR_BYTES, f.k_ratio);
                 if (lane == 0) mbar_arrive(sh.k_full + st);
@@ -431,7 +452,7 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                 put(vc, v_ring + st * TENSOR_BYTES, f.v_ratio);
                 if (lane == 0) mbar_arrive(sh.v_full + st);
                 ask(vc, a.v_cache, b + 1);
-                put_ratios(b + 1, page1, ks1, vs1);      // (here rather than at the loop's start, which delays the keys: 146 us instead of 150 in the case above)
+                put_ratios(b + 1, page1, ks1, vs1);      // (here rather than at the loop's start, which delays the keys: 4 us less in the case above)
                 put_info(b + 2, page2, ks, vs);
                 page1 = page2; ks1 = ks; vs1 = vs;
                 page2 = page3;
@@ -525,19 +546,26 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                 fence_after();
                 const int key0 = (block0 + b) * KEYS;
                 const BlockInfo& f = sh.info[b % INFO];
-                const bool even = f.even != 0;
+                const int kind = f.kind;
                 // (never zero: a hidden score of -inf has to stay one)
-                const float factor = fmaxf(row_factor * f.factor, 1e-37f), shift = f.shift;
+                const float factor = fmaxf(row_factor * (kind == EVEN ? f.factor : 1.f), 1e-37f), shift = f.shift;
                 // Rows without a token or head see what comes (their queries are zero); the others see keys row_lo .. row_pos.
                 const bool some_hidden = key0 < row_lo || key0 + KEYS - 1 > row_pos;
                 const int from = row_lo - key0;
                 const unsigned span = row_pos >= row_lo ? (unsigned)(row_pos - row_lo) : 0u;
                 auto hidden = [&](int j) { return (unsigned)(j - from) > span || row_pos < row_lo; };
-                if (even) {
+                auto in_registers = [&](auto by_key) {
+                    constexpr bool BY_KEY = decltype(by_key)::value;
                     uint32_t sv[KEYS / 32][32];
 #pragma unroll
                     for (int c = 0; c < KEYS / 32; ++c) ld32(tmem_s + (uint32_t)(c * 32), sv[c]);
                     wait_ld();
+                    if constexpr (BY_KEY) {      // each score by its key's scale
+#pragma unroll
+                        for (int c = 0; c < KEYS / 32; ++c)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) by_four(&sv[c][4 * i], reinterpret_cast<const float4*>(f.k_scale)[c * 8 + i]);
+                    }
                     if (some_hidden) {
 #pragma unroll
                         for (int c = 0; c < KEYS / 32; ++c)
@@ -564,8 +592,22 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                             unpair(fma2(pair_of(__uint_as_float(sv[c][2 * e]), __uint_as_float(sv[c][2 * e + 1])), factor2, off2), x0, x1);
                             const float p0 = exp2_of(x0), p1 = exp2_of(x1);
                             sum2[e & 3] = add2(sum2[e & 3], pair_of(p0, p1));
-                            const __half2 pk = __floats2half2_rn(p0, p1);
-                            pv[e] = *reinterpret_cast<const uint32_t*>(&pk);
+                            if constexpr (BY_KEY) {
+                                sv[c][2 * e] = __float_as_uint(p0);
+                                sv[c][2 * e + 1] = __float_as_uint(p1);
+                            } else {
+                                const __half2 pk = __floats2half2_rn(p0, p1);
+                                pv[e] = *reinterpret_cast<const uint32_t*>(&pk);
+                            }
+                        }
+                        if constexpr (BY_KEY) {      // each weight by its key's value scale over the largest
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) by_four(&sv[c][4 * i], reinterpret_cast<const float4*>(f.v_scale)[c * 8 + i]);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const __half2 pk = __floats2half2_rn(__uint_as_float(sv[c][2 * e]), __uint_as_float(sv[c][2 * e + 1]));
+                                pv[e] = *reinterpret_cast<const uint32_t*>(&pk);
+                            }
                         }
                         st16(tmem_s + (uint32_t)(c * 16), pv);
                     }
@@ -573,7 +615,10 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
 #pragma unroll
                     for (int i = 0; i < 4; ++i) { float x, z; unpair(sum2[i], x, z); sum4[i] = x + z; }
                     row.l += (double)(((sum4[0] + sum4[1]) + (sum4[2] + sum4[3])) * exp2_of(-shift - P_SHIFT));
-                } else {
+                };
+                if (kind == EVEN) in_registers(std::false_type{});
+                else if (kind == NEAR) in_registers(std::true_type{});
+                else {
                     row = one_by_one(f, tmem_s, tmem_o, row_factor, key0, row_lo, row_pos, b > 0, row);
                 }
                 wait_st();

@@ -136,3 +136,56 @@ def test_a_build_that_cannot_run_the_kernel_leaves_its_steps_to_the_other(status
 @pytest.mark.parametrize("zeros", ["first", "last", "all"])
 def test_blocks_of_zeros(status, case, lean, zeros):  # noqa: F811
     S.test_blocks_of_zeros(status, case, lean, zeros)
+
+
+def any_mantissa(b, seed):
+    gen = torch.Generator().manual_seed(seed)
+    b.ks *= 1 + torch.rand(b.ks.shape, generator=gen).cuda()
+    b.vs = (0.01 * (1 + 3 * torch.rand(b.vs.shape, generator=gen))).cuda()
+
+
+@by_size
+@pytest.mark.parametrize("seed", range(6))
+def test_scales_of_any_mantissa_within_2_to_the_4(status, case, seed):  # noqa: F811
+    """As a cache has them whose scales are a page's largest magnitude over 448. (A rounded ratio or product, 2^-11 of a score, would show.)"""
+    b = S.sizes(case, seed=seed, peak=6.0)
+    any_mantissa(b, seed)
+    b.check(status)
+    b.check(status, window=70)
+    b.ks[b.tables[0][3]] *= -1
+    b.ks[b.tables[1][2]] = 0
+    b.check(status)
+
+
+@by_size
+def test_values_of_zero_beside_key_scales_of_any_mantissa(status, case):  # noqa: F811
+    b = S.sizes(case, seed=3)
+    any_mantissa(b, 3)
+    b.vs.zero_()
+    got = b.run(status)
+    fine(status)
+    assert bool((got == 0).all())
+
+
+@by_size
+@pytest.mark.parametrize("power", [60, 70, 100, -100])
+def test_large_key_scales_and_small_queries(status, case, power):  # noqa: F811
+    b = S.sizes(case, seed=4)
+    any_mantissa(b, 4)
+    b.q = (b.q.float() * 2.0 ** -power).to(BF16)
+    b.ks *= 2.0 ** power
+    b.check(status)
+
+
+@by_size
+def test_mixed_kinds_of_blocks(status, case):  # noqa: F811
+    """Powers of two, any mantissas and scales far apart, 128 keys each and across."""
+    b = S.sizes(case, seed=5)
+    gen = torch.Generator().manual_seed(5)
+    for t in b.tables:
+        for i, p in enumerate(t):
+            kind = (i // 5) % 3
+            b.vs[p] = 0.01 * float(1 + torch.rand((), generator=gen)) if kind == 1 else 2.0 ** int(torch.randint(*((-7, -5) if kind == 0 else (-70, 20)), (), generator=gen))
+            b.ks[p] *= 1.0 if kind == 0 else float(1 + torch.rand((), generator=gen))
+    b.check(status)
+    b.check(status, window=90)
