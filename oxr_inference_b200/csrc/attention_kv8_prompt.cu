@@ -395,9 +395,9 @@ attn_kv8_prompt_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __r
                 top = fmaxf(top, shift);
                 if (page >= 0) {
                     const bool near = v_none || (vr >= 0.0625f && vr <= 1.00001f);
-                    const bool fits = k_exact || !(fabsf(ks) > 1.8e19f);      // 2^64: a score times it stays a float
-                    if (!(near && fits && fabsf(shift) <= 60.f && shift >= top - 60.f)) atomicMin(&f.kind, ODD);
-                    else if (!k_exact || !v_exact) atomicMin(&f.kind, NEAR);
+                    const bool fits = !(fmaxf(km, fabsf(ks)) > 1.8e19f);      // 2^64: a score times it stays a float
+                    if (!(near && fabsf(shift) <= 60.f && shift >= top - 60.f)) atomicMin(&f.kind, ODD);
+                    else if (!k_exact || !v_exact) atomicMin(&f.kind, fits ? NEAR : ODD);
                 }
                 if (lt == 0) {
                     f.factor = km > 0.f ? km : 1.f;

@@ -175,6 +175,8 @@ def test_large_key_scales_and_small_queries(status, case, power):  # noqa: F811
     b.q = (b.q.float() * 2.0 ** -power).to(BF16)
     b.ks *= 2.0 ** power
     b.check(status)
+    b.ks = S.powers(torch.full(tuple(b.ks.shape), power - 8.0))       # the same with keys that are powers of two
+    b.check(status)
 
 
 @by_size
